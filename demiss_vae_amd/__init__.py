@@ -6,3 +6,4 @@ from .mlp import NetDims, PackedNet, GeneratedDropout, ResidualMLPFunction, mlp_
 from .objectives import (ModelDims, estimate_elbo, estimate_iwelbo, estimate_multiple_elbo,  # noqa: F401
                          estimate_multiple_iwelbo, mvb2_objectives, cvi_objective, mvb_objective)
 from .graph import GraphedStep  # noqa: F401
+from .categorical import CategoricalLogProb, categorical_log_prob, distill_top_logits  # noqa: F401

@@ -17,6 +17,8 @@ IN_PLAIN, IN_MASKED, IN_CONCAT, IN_CONCAT_MASKED = 0, 1, 2, 3
 GEN = {"normal": 0, "normal_with_eps": 1, "bern": 2, "bern_m1_p1": 3}
 Q_OWN, Q_STRATIFIED, Q_IMPUTATION = 0, 1, 2
 BOUND_LSE, BOUND_WEIGHTED, BOUND_PER_COMPONENT, TERMS_ONLY = 0, 1, 2, -1
+CAT_DTYPE = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+CAT_MAX_TOP, CAT_MAX_TEACHER, CAT_SHORT_ROW = 64, 256, 1024
 E_BADARG, E_UNSUPPORTED, E_WORKSPACE = -1, -2, -3
 
 
@@ -63,6 +65,17 @@ class DmvObjFwd(C.Structure):
 class DmvPackMap(C.Structure):
     _fields_ = [("image", C.c_void_p), ("fwd_off", C.c_int64), ("tr_off", C.c_int64), ("N", C.c_int32), ("K", C.c_int32),
                 ("S", C.c_int32), ("Sn", C.c_int32), ("is_bias", C.c_int32), ("reserved", C.c_int32)]
+
+
+class DmvCatRows(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("rows", C.c_int64), ("V", C.c_int32), ("dtype", C.c_int32),
+                ("X", C.c_void_p), ("x_period", C.c_int64), ("M", C.c_void_p), ("m_period", C.c_int64),
+                ("sizes", C.c_void_p), ("size_period", C.c_int64)]
+
+
+class DmvCatTeacher(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("index", C.c_void_p), ("period", C.c_int64), ("k", C.c_int32), ("dtype", C.c_int32),
+                ("weight", C.c_void_p), ("w_period", C.c_int64), ("temperature", C.c_float)]
 
 
 class DmvAdamGroup(C.Structure):
@@ -138,6 +151,12 @@ SIGNATURES = {
     "dmv_rows_scatter": (C.c_int, [_P, _P, _I64, _I32, _P, _P]),
     "dmv_impute_tail": (C.c_int, [_I64, _I32, _I32, _P, _I64, _P, _P, _P, _P, _U64, _U64, _P, _P, _P, _I32, _P, _P, _P, _P]),
     "dmv_categorical_draw": (C.c_int, [_I32, _I32, _I32, _P, _P, _U64, _U64, _P, _P, _P]),
+    "dmv_cat_log_prob_ws_bytes": (_SZ, [C.POINTER(DmvCatRows), _I32]),
+    "dmv_cat_log_prob": (C.c_int, [C.POINTER(DmvCatRows), _P, _P, _I32, _P, _P, _P, _P, _SZ, _P]),
+    "dmv_cat_log_prob_backward": (C.c_int, [C.POINTER(DmvCatRows), _P, _P, _P, _I32, _P, _P, _P, _I64, _P]),
+    "dmv_cat_distill_ws_bytes": (_SZ, [C.POINTER(DmvCatRows)]),
+    "dmv_cat_distill": (C.c_int, [C.POINTER(DmvCatRows), C.POINTER(DmvCatTeacher), _P, _P, _P, _P, _I64, _P, _SZ, _P]),
+    "dmv_cat_distill_backward": (C.c_int, [C.POINTER(DmvCatRows), C.POINTER(DmvCatTeacher), _P, _I32, _P, _P, _I64, _P]),
     "dmv_lair_row_map": (C.c_int, [_I32, _I32, _I32, _P, _P, _P]),
     "dmv_dropout_masks": (C.c_int, [_P, _I64, _F, _U64, _U64, _P, _P]),
     "dmv_clock_watch": (C.c_int, [_I64, _P, _P]),

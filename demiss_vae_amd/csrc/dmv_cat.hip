@@ -1,0 +1,1674 @@
+// Categorical rows: log-probabilities of given categories with the row's entropy and its most probable alternatives, the
+// gradient of those, and distillation from a teacher's top logits (loss and gradient).
+//
+// A row is n <= V logits x of one categorical entry.  With c = log2(e) / T, m = max x and d_v = c (x_v - m):
+//   s = sum_v 2^d_v = 1 + r,   log q_v = ln2 d_v - log1p(r),   H = log1p(r) + ln2 u / s,   u = -sum_v 2^d_v d_v.
+// r and u are sums over the categories OTHER than the largest one (its terms are 1 and 0 exactly), so a row that is
+// nearly certain of one category keeps the relative accuracy of its log-probability and entropy: 1 + r would round r to
+// 6e-8.  Partial results (of a thread, a workgroup, a part of a row) carry (m, s or r, u) and are joined by rescaling
+// with 2^(c (m_part - m)).  All sums are held in 32 bits, the sum of the losses of all rows in 64.
+#include "dmv_common.h"
+#include "dmv_objmath.h"
+
+#include <type_traits>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kClampD = -256.f;        // 2^d is 0 below: keeps 0 * (-inf) out of the entropy sum
+constexpr float kNearCertain = 0.0625f;  // below this r the largest category's thread sums its other terms again
+constexpr int kMaxTop = DMV_CAT_MAX_TOP;
+constexpr int kMaxTeacher = DMV_CAT_MAX_TEACHER;
+
+// ------------------------------------------------------------------------------------------ elements
+// 16 bytes of a row whose address is only element-aligned: one 16-byte access (the hardware takes any alignment)
+struct __attribute__((packed, aligned(2))) Raw16 {
+  uint32_t w[4];
+};
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<DMV_F32> {
+  typedef float type;
+  static constexpr int N = 4;
+  static constexpr int kOpenBits = 0;    // low bits of an order key that no two values of the type differ in alone
+  static __device__ __forceinline__ float load(const void* p, int64_t i) { return ((const float*)p)[i]; }
+  static __device__ __forceinline__ void store(void* p, int64_t i, float v) { ((float*)p)[i] = v; }
+  static __device__ __forceinline__ void unpack(const Raw16& r, float* v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(r.w[e]);
+  }
+  static __device__ __forceinline__ void pack(const float* v, Raw16& r) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.w[e] = __float_as_uint(v[e]);
+  }
+};
+template <>
+struct Elem<DMV_BF16> {
+  typedef uint16_t type;
+  static constexpr int N = 8;
+  static constexpr int kOpenBits = 16;
+  static __device__ __forceinline__ float load(const void* p, int64_t i) {
+    return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t i, float v) { ((__bf16*)p)[i] = (__bf16)v; }
+  static __device__ __forceinline__ void unpack(const Raw16& r, float* v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(r.w[e] << 16);
+      v[2 * e + 1] = __uint_as_float(r.w[e] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ void pack(const float* v, Raw16& r) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      r.w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){v[2 * e], v[2 * e + 1]}, bf16x2_t));
+  }
+};
+template <>
+struct Elem<DMV_F16> {
+  typedef _Float16 type;
+  static constexpr int N = 8;
+  static constexpr int kOpenBits = 13;
+  static __device__ __forceinline__ float load(const void* p, int64_t i) { return (float)((const _Float16*)p)[i]; }
+  static __device__ __forceinline__ void store(void* p, int64_t i, float v) { ((_Float16*)p)[i] = (_Float16)v; }
+  static __device__ __forceinline__ void unpack(const Raw16& r, float* v) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const h2 h = __builtin_bit_cast(h2, r.w[e]);
+      v[2 * e] = (float)h[0];
+      v[2 * e + 1] = (float)h[1];
+    }
+  }
+  static __device__ __forceinline__ void pack(const float* v, Raw16& r) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.w[e] = __builtin_bit_cast(uint32_t, (h2){(_Float16)v[2 * e], (_Float16)v[2 * e + 1]});
+  }
+};
+static inline int elem_size(int dt) { return dt == DMV_F32 ? 4 : 2; }
+static inline int vec_elems(int dt) { return dt == DMV_F32 ? 4 : 8; }
+
+// Order of the selection: larger values first, lower index first among equal ones (-0 and +0 are equal).  The key grows
+// with the value; a 16-bit value's key is determined by its upper half.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+constexpr uint32_t kKeyMinusInf = 0x007fffffu;  // order_key(-inf)
+
+// max(a, b, c) in one instruction; what is NaN is left out (fmaxf costs another instruction per operand whose origin the
+// compiler does not know)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ float max_of(const float* v, float m) {
+  if constexpr (N == 1) return max3(v[0], m, m);
+#pragma unroll
+  for (int e = 0; e + 1 < N; e += 2) m = max3(v[e], v[e + 1], m);
+  return m;
+}
+
+__device__ __forceinline__ float exp2_hw(float d) { return __builtin_amdgcn_exp2f(d); }
+
+template <int R>
+__device__ __forceinline__ float gmax(float v) {
+  if (R >= 2) v = fmaxf(v, dpp_move<0xB1>(v));
+  if (R >= 4) v = fmaxf(v, dpp_move<0x4E>(v));
+  if (R >= 8) v = fmaxf(v, dpp_move<0x141>(v));
+  if (R >= 16) v = fmaxf(v, dpp_move<0x140>(v));
+  if (R >= 32) v = fmaxf(v, __shfl_xor(v, 16));
+  if (R >= 64) v = fmaxf(v, __shfl_xor(v, 32));
+  return v;
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_move_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int R>
+__device__ __forceinline__ uint32_t gmax_u(uint32_t v) {
+  if (R >= 2) v = max(v, dpp_move_u<0xB1>(v));
+  if (R >= 4) v = max(v, dpp_move_u<0x4E>(v));
+  if (R >= 8) v = max(v, dpp_move_u<0x141>(v));
+  if (R >= 16) v = max(v, dpp_move_u<0x140>(v));
+  if (R >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  if (R >= 64) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------ arguments
+struct Rows {
+  const char* x;
+  int64_t ld, rows;  // pitch in elements
+  int V;
+  const int64_t* X;
+  const uint8_t* M;
+  const int32_t* sizes;
+  int64_t x_period, m_period, size_period;
+};
+
+// entry of a per-row array that repeats with `period` rows
+__device__ __forceinline__ int64_t wrap(int64_t row, int64_t period, int64_t rows) {
+  if (period == rows) return row;
+  if ((uint64_t)rows <= 0xffffffffull) return (int64_t)((uint32_t)row % (uint32_t)period);
+  return row % period;
+}
+__device__ __forceinline__ int row_size(const Rows& a, int64_t row) {
+  if (!a.sizes) return a.V;
+  const int n = a.sizes[wrap(row, a.size_period, a.rows)];
+  return n < 0 ? 0 : (n > a.V ? a.V : n);
+}
+__device__ __forceinline__ bool row_seen(const Rows& a, int64_t row) { return !a.M || a.M[wrap(row, a.m_period, a.rows)] != 0; }
+
+struct Fwd {
+  Rows r;
+  float* log_prob;
+  float* entropy;
+  int top;
+  float* top_lp;
+  int64_t* top_idx;
+  f32x4* stats;  // per row (m, 1 / s, log s, H): what the gradient reads; 1 / s = 0: nothing of non-zero probability
+  float c;       // log2(e) / T
+  int parts;     // workgroups per row; > 1: partial results go to ws
+  f32x4* part;   // [rows][parts] (m, r, u, -)
+  uint2* part_top;  // [rows][parts][top] (key, index), in order; key 0 past the end
+};
+
+struct Bwd {
+  Rows r;
+  const f32x4* stats;
+  const float* g_lp;
+  const float* g_ent;
+  int top;
+  const int64_t* top_idx;
+  const float* g_top;
+  void* d;
+  int64_t ld_d;
+  int chunks;
+};
+
+struct Teacher {
+  const void* t;
+  const int64_t* idx;
+  const float* weight;
+  int64_t t_period, w_period;
+  int k, dt;
+  float c;      // log2(e) / T
+  float inv_T;
+};
+
+struct Dist {
+  Rows r;
+  Teacher t;
+  float* per_row;
+  double* loss_part;  // one per workgroup of the launch
+  f32x4* stats;
+  const float* gscale;
+  int unless_one;  // the gradient of gscale = 1 is already in place
+  void* d;         // nullable: loss only
+  int64_t ld_d;
+  int chunks, parts;
+  f32x4* part;
+};
+
+__device__ __forceinline__ float teacher_logit(const Teacher& t, int64_t i) {
+  if (t.dt == DMV_F32) return Elem<DMV_F32>::load(t.t, i);
+  if (t.dt == DMV_BF16) return Elem<DMV_BF16>::load(t.t, i);
+  return Elem<DMV_F16>::load(t.t, i);
+}
+
+// Slot `s` of a row = its elements [s VEC, s VEC + VEC).  The access starts at min(s VEC, V - VEC), so it never leaves the
+// row (V >= VEC): the last slot of a row whose length is no multiple of VEC overlaps the one before.
+template <int VEC>
+__device__ __forceinline__ int slot_base(int s, int V) {
+  const int b = s * VEC;
+  return b + VEC <= V ? b : V - VEC;
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void slot_load(const char* row, int base, float* v) {
+  if constexpr (VEC == 1) {
+    v[0] = Elem<DT>::load(row, base);
+  } else {
+    static_assert(VEC == Elem<DT>::N, "");
+    Elem<DT>::unpack(*(const Raw16*)(row + (int64_t)base * (int)sizeof(typename Elem<DT>::type)), v);
+  }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void slot_store(char* row, int base, const float* v) {
+  if constexpr (VEC == 1) {
+    Elem<DT>::store(row, base, v[0]);
+  } else {
+    Raw16 r;
+    Elem<DT>::pack(v, r);
+    *(Raw16*)(row + (int64_t)base * (int)sizeof(typename Elem<DT>::type)) = r;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ gradient of one row
+// With S = g_lp + sum_j g_top[j] and a_v what of S belongs to category v itself:
+//   dx_v = a_v - S q_v - g_H q_v (log q_v + H)
+// The dense part (a_v = 0) is written for every category; the few with a_v != 0 are written again by `at`, with
+// a_v (1 - q_v) as -a_v expm1(log q_v): no cancellation where q_v is close to 1.
+struct RowGrad {
+  float m, inv_s, logs, S, gh, H;
+  __device__ __forceinline__ float dense(float x) const {
+    const float y = x - m;
+    const float q = exp2_hw(y * kLog2e) * inv_s;
+    return -q * (S + gh * (fmaxf(y - logs, -1e30f) + H));
+  }
+  __device__ __forceinline__ float at(float x, float a) const {
+    const float lq = fmaxf(x - m - logs, -1e30f);
+    const float q = exp2_hw(lq * kLog2e);
+    return -a * expm1f(lq) - (S - a) * q - gh * q * (lq + H);
+  }
+};
+
+// ------------------------------------------------------------------------------------------ short rows
+// L lanes hold a row of up to 16 L elements in registers (SL slots of VEC elements each); 64 / L rows per wavefront.
+constexpr int kSmallThreads = 256;
+
+template <int DT, int VEC, int L, int SL>
+struct SmallRow {
+  static constexpr int E = VEC * SL;
+  float v[E];
+  int n, lane;
+  const char* p;
+  // element e of this lane: its index in the row, and whether it counts (each category exactly once, below n)
+  __device__ __forceinline__ int first(int j) const { return (lane + L * j) * VEC; }
+  __device__ __forceinline__ void load(const Rows& a, int64_t row, int lane_, int n_) {
+    lane = lane_;
+    n = n_;
+    p = a.x + row * a.ld * (int64_t)sizeof(typename Elem<DT>::type);
+#pragma unroll
+    for (int j = 0; j < SL; ++j) {
+      if (first(j) < a.V) {
+        slot_load<DT, VEC>(p, slot_base<VEC>(lane + L * j, a.V), v + j * VEC);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[j * VEC + e] = -INFINITY;
+      }
+    }
+  }
+  // the elements that do not count become -inf
+  __device__ __forceinline__ void counted(int V, float* o) const {
+#pragma unroll
+    for (int j = 0; j < SL; ++j) {
+      const int b = slot_base<VEC>(lane + L * j, V), f = first(j);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int i = b + e;
+        o[j * VEC + e] = (i >= f && i < n) ? v[j * VEC + e] : -INFINITY;
+      }
+    }
+  }
+};
+
+// (m, r, u) of a row held by L lanes; r < 0: no category of non-zero probability
+template <int L, int E>
+__device__ __forceinline__ void small_stats(const float* o, float c, bool entropy, float& m, float& r, float& u) {
+  m = gmax<L>(max_of<E>(o, -INFINITY));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float d = (o[e] - ref) * c, w = exp2_hw(d);
+    s += w;
+    if (entropy) t = fmaf(w, fmaxf(d, kClampD), t);
+  }
+  r = gsum<L>(s) - 1.f;
+  u = entropy ? -gsum<L>(t) : 0.f;
+  if (r < kNearCertain && r >= 0.f) {
+    s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += o[e] < m ? exp2_hw((o[e] - m) * c) : 0.f;
+    r = gsum<L>(s);
+  }
+}
+
+template <int DT, int VEC, int L, int SL>
+__global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
+  constexpr int E = VEC * SL;
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t row = (int64_t)blockIdx.x * (kSmallThreads / L) + threadIdx.x / L;
+  if (row >= a.r.rows) return;
+  const bool seen = row_seen(a.r, row);
+  if (!seen && !a.entropy && !a.top) {
+    if (lane == 0 && a.log_prob) a.log_prob[row] = 0.f;
+    return;
+  }
+  const int n = row_size(a.r, row);
+  SmallRow<DT, VEC, L, SL> x;
+  x.load(a.r, row, lane, n);
+  int64_t X = -1;
+  float xX = -INFINITY;
+  if (a.log_prob && seen) {
+    X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
+    if (X >= 0 && X < n) xX = Elem<DT>::load(x.p, X);
+  }
+  float o[E], m, r, u;
+  x.counted(a.r.V, o);
+  small_stats<L, E>(o, a.c, a.entropy != nullptr, m, r, u);
+  const bool empty = m == -INFINITY && !(r != r);
+  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
+  if (lane == 0) {
+    if (a.log_prob) {
+      float lp = 0.f;
+      if (seen) lp = (X < 0 || X >= n) ? NAN : (empty ? -INFINITY : (xX - m) - logs);
+      a.log_prob[row] = lp;
+    }
+    if (a.entropy) a.entropy[row] = H;
+    if (a.stats) a.stats[row] = f32x4{m, inv_s, logs, H};
+  }
+  if (a.top) {
+    const bool bad = logs != logs;
+    uint32_t k[E];
+#pragma unroll
+    for (int j = 0; j < SL; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float w = o[j * VEC + e];
+        k[j * VEC + e] = (w > -INFINITY) ? order_key(w) : 0u;
+      }
+    for (int t = 0; t < a.top; ++t) {
+      uint32_t best = 0;
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int j = 0; j < SL; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const uint32_t w = k[j * VEC + e];
+          if (w > best) {
+            best = w;
+            at = slot_base<VEC>(lane + L * j, a.r.V) + e;
+          }
+        }
+      const uint32_t top = gmax_u<L>(best);
+      const uint32_t low = ~gmax_u<L>(best == top ? ~(uint32_t)at : 0u);   // lowest index among the equal ones
+#pragma unroll
+      for (int j = 0; j < SL; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (slot_base<VEC>(lane + L * j, a.r.V) + e == (int)low) k[j * VEC + e] = 0u;
+      if (lane == (t & (L - 1))) {
+        const int64_t at_out = row * a.top + t;
+        const bool none = top == 0u || bad;
+        a.top_idx[at_out] = none ? -1 : (int64_t)low;
+        a.top_lp[at_out] = bad ? NAN : (none ? -INFINITY : (key_value(top) - m) - logs);
+      }
+    }
+  }
+}
+
+// a_v of the gradient's sparse part for category v: what of the given category and the top alternatives falls on it
+__device__ __forceinline__ float own_share(const Bwd& a, int64_t row, int64_t v, int64_t X, float gl) {
+  float s = v == X ? gl : 0.f;
+  if (a.g_top)
+    for (int j = 0; j < a.top; ++j)
+      if (a.top_idx[row * a.top + j] == v) s += a.g_top[row * a.top + j];
+  return s;
+}
+
+// S of a row (and its given category, -1 if none), the same in every lane of the R lanes that ask
+template <int R>
+__device__ __forceinline__ RowGrad row_grad(const Bwd& a, int64_t row, int lane, int n, int64_t& X, float& gl) {
+  RowGrad g;
+  X = -1;
+  gl = 0.f;
+  if (a.g_lp && row_seen(a.r, row)) {
+    X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
+    gl = a.g_lp[row];
+    if (X < 0 || X >= n) gl = NAN;      // as the log-probability of no category at all
+  }
+  g.S = gl;
+  if (a.g_top) {
+    float s = 0.f;
+    for (int j = lane; j < a.top; j += R)
+      if (a.top_idx[row * a.top + j] >= 0) s += a.g_top[row * a.top + j];
+    g.S += gsum<R>(s);
+  }
+  g.gh = a.g_ent ? a.g_ent[row] : 0.f;
+  g.m = g.inv_s = g.logs = g.H = 0.f;
+  if (g.S != 0.f || g.gh != 0.f || a.g_top) {
+    const f32x4 st = a.stats[row];
+    g.m = st[0], g.inv_s = st[1], g.logs = st[2], g.H = st[3];
+  }
+  return g;
+}
+
+template <int DT, int VEC, int L, int SL>
+__global__ void __launch_bounds__(kSmallThreads) k_cat_bwd_small(Bwd a) {
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t row = (int64_t)blockIdx.x * (kSmallThreads / L) + threadIdx.x / L;
+  if (row >= a.r.rows) return;
+  const int n = row_size(a.r, row), V = a.r.V;
+  int64_t X;
+  float gl;
+  const RowGrad g = row_grad<L>(a, row, lane, n, X, gl);
+  char* out = (char*)a.d + row * a.ld_d * (int64_t)sizeof(typename Elem<DT>::type);
+  const bool live = (g.S != 0.f || g.gh != 0.f || a.g_top) && g.inv_s != 0.f;
+  SmallRow<DT, VEC, L, SL> x;
+  if (live) x.load(a.r, row, lane, n);
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    const int f = (lane + L * j) * VEC;
+    if (f >= V) continue;
+    const int b = slot_base<VEC>(lane + L * j, V);
+    float o[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = (live && b + e < n) ? g.dense(x.v[j * VEC + e]) : 0.f;
+    slot_store<DT, VEC>(out, b, o);
+  }
+  if (!live) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // the dense part before the few categories written again
+  __builtin_amdgcn_wave_barrier();
+  const int entries = 1 + (a.g_top ? a.top : 0);
+  for (int j = lane; j < entries; j += L) {
+    const int64_t v = j == 0 ? X : a.top_idx[row * a.top + j - 1];
+    if (v < 0 || v >= n) continue;
+    Elem<DT>::store(out, v, g.at(Elem<DT>::load(x.p, v), own_share(a, row, v, X, gl)));
+  }
+}
+
+// ------------------------------------------------------------------------------------------ distillation, shared parts
+// Teacher entry j counts if its index is not negative and its logit not -inf; the counted ones are normalised among
+// themselves.  An index past the row's categories, or a logit that is NaN or +inf, makes the row's loss and gradient NaN.
+__device__ __forceinline__ bool entry_counts(float t, int64_t i) { return i >= 0 && t != -INFINITY; }
+
+template <int DT>
+struct Student {
+  float m, inv_s, logs, c, inv_T;
+  const char* p;
+  // log q of category v (any rounding of the sum near 1 is already in logs)
+  __device__ __forceinline__ float log_q(int64_t v) const { return (Elem<DT>::load(p, v) - m) * inv_T - logs; }
+  __device__ __forceinline__ float q(float x) const { return exp2_hw((x - m) * c) * inv_s; }
+};
+
+// q - p without its cancellation
+__device__ __forceinline__ float q_minus_p(float lq, float p) {
+  const float q = expf(lq);
+  if (p > 0.5f * q) return p * expm1f(lq - logf(p));
+  return q - p;
+}
+
+template <int DT, int VEC, int L, int SL>
+__global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
+  constexpr int E = VEC * SL;
+  __shared__ double sums[kSmallThreads / 64];
+  const float gs = a.gscale ? *a.gscale : 1.f;
+  if (a.unless_one && gs == 1.f) return;
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t row = (int64_t)blockIdx.x * (kSmallThreads / L) + threadIdx.x / L;
+  float kl = 0.f, w = 0.f;
+  if (row < a.r.rows) {
+    const int n = row_size(a.r, row), V = a.r.V, K = a.t.k;
+    w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
+    SmallRow<DT, VEC, L, SL> x;
+    Student<DT> st;
+    bool any = false, bad = false, empty = true;
+    float tm = -INFINITY, t_logs = 0.f;
+    const int64_t t0 = wrap(row, a.t.t_period, a.r.rows) * K;
+    if (w != 0.f) {
+      x.load(a.r, row, lane, n);
+      for (int j = lane; j < K; j += L) {
+        const int64_t i = a.t.idx[t0 + j];
+        const float t = teacher_logit(a.t, t0 + j);
+        if (!entry_counts(t, i)) continue;
+        any = true;
+        bad = bad || i >= n || !(t < INFINITY);
+        tm = fmaxf(tm, t);
+      }
+      tm = gmax<L>(tm);
+      any = gmax<L>(any ? 1.f : 0.f) > 0.f;
+      bad = gmax<L>(bad ? 1.f : 0.f) > 0.f;
+      float s = 0.f, held = 0.f;
+      for (int j = lane; j < K; j += L) {
+        const int64_t i = a.t.idx[t0 + j];
+        const float t = teacher_logit(a.t, t0 + j);
+        if (!entry_counts(t, i)) continue;
+        if (t == tm) held += 1.f;
+        else s += exp2_hw((t - tm) * a.t.c);
+      }
+      t_logs = log1pf(gsum<L>(s) + (gsum<L>(held) - 1.f));
+      float o[E], m, r, u;
+      x.counted(V, o);
+      small_stats<L, E>(o, a.t.c, false, m, r, u);
+      empty = m == -INFINITY && !(r != r);
+      st.m = m, st.c = a.t.c, st.inv_T = a.t.inv_T, st.p = x.p;
+      st.logs = empty ? 0.f : log1pf(r);
+      st.inv_s = empty ? 0.f : 1.f / (1.f + r);
+      if (lane == 0 && a.stats) a.stats[row] = f32x4{st.m, st.inv_s, st.logs, 0.f};
+      if (any && !bad && !empty) {
+        for (int j = lane; j < K; j += L) {
+          const int64_t i = a.t.idx[t0 + j];
+          const float t = teacher_logit(a.t, t0 + j);
+          if (!entry_counts(t, i)) continue;
+          const float lp = (t - tm) * a.t.inv_T - t_logs, p = expf(lp);
+          if (p > 0.f) kl += p * (lp - st.log_q(i));
+        }
+      }
+      kl = gsum<L>(kl);
+      if (any && empty) kl = INFINITY;
+      if (bad) kl = NAN;
+    }
+    if (lane == 0 && a.per_row) a.per_row[row] = kl;
+    if (a.d) {
+      char* out = (char*)a.d + row * a.ld_d * (int64_t)sizeof(typename Elem<DT>::type);
+      const bool live = w != 0.f && any && !empty;
+      const float scale = bad ? NAN : gs * w * a.t.inv_T;
+#pragma unroll
+      for (int j = 0; j < SL; ++j) {
+        const int f = (lane + L * j) * VEC;
+        if (f >= V) continue;
+        const int b = slot_base<VEC>(lane + L * j, V);
+        float g[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] = (live && b + e < n) ? scale * st.q(x.v[j * VEC + e]) : 0.f;
+        slot_store<DT, VEC>(out, b, g);
+      }
+      if (live && !bad) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        for (int j = lane; j < K; j += L) {
+          const int64_t i = a.t.idx[t0 + j];
+          if (!entry_counts(teacher_logit(a.t, t0 + j), i)) continue;
+          float p = 0.f;      // the same category may be given more than once
+          for (int h = 0; h < K; ++h)
+            if (a.t.idx[t0 + h] == i) p += expf((teacher_logit(a.t, t0 + h) - tm) * a.t.inv_T - t_logs);
+          Elem<DT>::store(out, i, scale * q_minus_p(st.log_q(i), p));
+        }
+      }
+    }
+  }
+  // the workgroup's share of the loss, in a fixed order
+  double part = (lane == 0 && w != 0.f) ? (double)w * (double)kl : 0.0;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) part += __shfl_xor(part, off);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = part;
+  __syncthreads();
+  if (threadIdx.x == 0 && a.loss_part) {
+    double s = 0.0;
+    for (int i = 0; i < kSmallThreads / 64; ++i) s += sums[i];
+    a.loss_part[blockIdx.x] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ long rows
+template <int NT>
+struct BlockRed {
+  float x[3][NT / 64];
+};
+template <int NT>
+__device__ __forceinline__ float block_max(float v, BlockRed<NT>& s) {
+  v = gmax<64>(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.x[0][threadIdx.x >> 6] = v;
+  __syncthreads();
+  float m = s.x[0][0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, s.x[0][i]);
+  return m;
+}
+template <int NT>
+__device__ __forceinline__ void block_sum3(float& p, float& q, float& w, BlockRed<NT>& s) {
+  p = gsum<64>(p), q = gsum<64>(q), w = gsum<64>(w);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    s.x[0][threadIdx.x >> 6] = p;
+    s.x[1][threadIdx.x >> 6] = q;
+    s.x[2][threadIdx.x >> 6] = w;
+  }
+  __syncthreads();
+  p = q = w = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) p += s.x[0][i], q += s.x[1][i], w += s.x[2][i];
+}
+
+// running (max, sum, entropy sum) of one thread
+struct Online {
+  float m = -INFINITY, s = 0.f, t = 0.f;
+  template <int N, bool ENT>
+  __device__ __forceinline__ void add(const float* v, float c) {
+    const float mn = max_of<N>(v, m);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float shift = fmaxf((m - ref) * c, kClampD), f = exp2_hw(shift);
+    if (ENT) t = f * fmaf(s, shift, t);
+    s *= f;
+    m = mn;
+    float s1 = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float d0 = (v[e] - ref) * c, w0 = exp2_hw(d0);
+      const float d1 = (v[e + 1] - ref) * c, w1 = exp2_hw(d1);
+      s += w0;
+      s1 += w1;
+      if (ENT) {
+        t = fmaf(w0, fmaxf(d0, kClampD), t);
+        t1 = fmaf(w1, fmaxf(d1, kClampD), t1);
+      }
+    }
+    s += s1;
+    if (ENT) t += t1;
+  }
+};
+
+// Joins the threads' partial results; on return (m, r, u) are the same in every thread.
+//   resum(holder): sum over x < m of 2^(c (x - m)) over this thread's share of the elements that thread `holder` had
+template <int NT, bool ENT, typename ReSum>
+__device__ __forceinline__ void block_join(const Online& on, float c, BlockRed<NT>& red, int* holder, float& m, float& r, float& u,
+                                           ReSum resum) {
+  m = block_max<NT>(on.m, red);
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float shift = fmaxf((on.m - ref) * c, kClampD), f = exp2_hw(shift);
+  const bool holds = on.m == m;
+  const float mine = holds ? on.s - 1.f : on.s * f;
+  float a = mine, b = ENT ? -f * fmaf(on.s, shift, on.t) : 0.f, h = holds ? 1.f : 0.f;
+  if (holds) *holder = threadIdx.x;
+  block_sum3<NT>(a, b, h, red);
+  r = a + (h - 1.f);
+  u = b;
+  if (m == -INFINITY && !(r != r)) r = -1.f;      // nothing of non-zero probability
+  else if (r < kNearCertain) {                    // one thread holds the largest: its sum has rounded the rest away
+    float again = resum(*holder, ref) + (holds ? 0.f : mine), z0 = 0.f, z1 = 0.f;
+    block_sum3<NT>(again, z0, z1, red);
+    r = again;
+  }
+}
+
+constexpr int kRowThreads = 256;
+constexpr int kUnroll = 4;              // slots in flight per thread
+constexpr int kGroups = 16;             // slot groups whose maxima a thread keeps for the selection
+constexpr int kCand = 1024;             // candidates of a selection
+
+template <int DT, bool TOP>
+struct RowShared {
+  BlockRed<kRowThreads> red;
+  int holder;
+};
+template <int DT>
+struct TopShared {
+  float gm[kGroups][kRowThreads];
+  float tmax[kRowThreads];
+  uint2 cand[kCand];
+  int count;
+  unsigned long long best[kRowThreads / 64];
+  int scan[kRowThreads / 64];
+};
+
+// The selection's result goes through `emit(rank, key, index)`.
+//
+// Every thread knows the largest value of each of its slot groups.  tau, the k-th largest of the threads' largest values
+// (256 of them), is a lower bound of the k-th largest element, and only the groups whose largest value reaches it are read
+// again: about k (1 + k / 512) elements of an ordinary row.  They are ranked by counting.  Rows with more candidates
+// than fit (many equal values) take the ordered scan below, and in the worst case one pass over the row per rank.
+template <int DT, int VEC, typename Emit>
+__device__ void block_top(TopShared<DT>& sh, const char* p, int V, int n, int s0, int s1, int gsz, int k, float tmax, Emit emit) {
+  constexpr int NT = kRowThreads;
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) sh.count = 0;
+  sh.tmax[tid] = tmax;
+  __syncthreads();
+  uint32_t g[NT / 64];
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) g[w] = order_key(sh.tmax[64 * w + lane]);
+  // largest t with count(key >= t) >= k, bit by bit, down to the bits that differ between values of the type
+  uint32_t tau = 0;
+  for (int bit = 31; bit >= Elem<DT>::kOpenBits; --bit) {
+    const uint32_t t = tau | (1u << bit);
+    int cnt = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) cnt += __popcll(__ballot(g[w] >= t));
+    if (cnt >= k) tau = t;
+    if (cnt == k) break;
+  }
+  if (tau <= kKeyMinusInf) tau = kKeyMinusInf + 1;   // -inf is no alternative
+  auto each = [&](uint32_t lowest, auto f) {          // f(key, index) of this thread's elements with key >= lowest
+    if (order_key(tmax) < lowest) return;
+    const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
+    for (int q = 0; q < groups; ++q) {
+      if (order_key(sh.gm[q][tid]) < lowest) continue;
+      for (int i = 0; i < gsz; ++i) {
+        const int s = s0 + tid + NT * (q * gsz + i);
+        if (s >= s1) break;
+        float v[VEC];
+        const int b = slot_base<VEC>(s, V);
+        slot_load<DT, VEC>(p, b, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const uint32_t key = order_key(v[e]);
+          if (b + e >= s * VEC && b + e < n && key >= lowest) f(key, b + e);
+        }
+      }
+    }
+  };
+  auto collect = [&](uint32_t lowest) {
+    each(lowest, [&](uint32_t key, int i) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) sh.cand[at] = make_uint2(key, (uint32_t)i);
+    });
+    __syncthreads();
+    return sh.count;
+  };
+  auto rank_all = [&](int have) {                     // ranks of all candidates, those below k are emitted
+    for (int i = tid; i < have; i += NT) {
+      const uint2 me = sh.cand[i];
+      int rank = 0;
+      for (int j = 0; j < have; ++j) {
+        const uint2 o = sh.cand[j];
+        rank += (o.x > me.x || (o.x == me.x && o.y < me.y)) ? 1 : 0;
+      }
+      if (rank < k) emit(rank, me.x, (int)me.y);
+    }
+  };
+  int have = collect(tau);
+  int done;
+  if (have <= kCand) {
+    rank_all(have);
+    done = have;
+  } else {
+    // many values reach tau: make it the key of the k-th largest of the threads' values itself, so that those equal to
+    // it can be told from those above
+    uint32_t kth = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) kth = (g[w] >= tau && g[w] < kth) ? g[w] : kth;
+    kth = ~gmax_u<64>(~kth);
+    if (kth != 0xffffffffu) tau = kth;
+    const uint32_t above = tau + 1u;
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    have = collect(above);
+    if (have <= kCand) {
+      rank_all(have);
+      done = have < k ? have : k;
+      // elements equal to tau, lowest index first: a round covers NT consecutive slots, in index order by thread
+      for (int it = 0; done < k && s0 + NT * it < s1; ++it) {
+        const int s = s0 + tid + NT * it;
+        uint32_t bits = 0, key0 = 0;
+        const int b = slot_base<VEC>(s < s1 ? s : s1 - 1, V);
+        if (s < s1) {
+          float v[VEC];
+          slot_load<DT, VEC>(p, b, v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const uint32_t key = order_key(v[e]);
+            if (b + e >= s * VEC && b + e < n && key >= tau && key < above) {
+              bits |= 1u << e;
+              key0 = key;
+            }
+          }
+        }
+        const int c = __popc(bits);
+        int before = 0;      // inclusive scan over the wavefront
+        int run = c;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int up = __shfl_up(run, off);
+          if (lane >= off) run += up;
+        }
+        before = run - c;
+        __syncthreads();
+        if (lane == 63) sh.scan[tid >> 6] = run;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+          if (w < (tid >> 6)) before += sh.scan[w];
+          total += sh.scan[w];
+        }
+        int rank = done + before;
+        for (int e = 0; e < VEC; ++e)
+          if ((bits >> e) & 1u) {
+            if (rank < k) emit(rank, key0, b + e);
+            ++rank;
+          }
+        done += total;
+      }
+    } else {
+      // one rank per pass: the best (key, lower index) after the last one
+      unsigned long long last = ~0ull;
+      for (done = 0; done < k; ++done) {
+        unsigned long long best = 0;
+        each(tau, [&](uint32_t key, int i) {
+          const unsigned long long o = ((unsigned long long)key << 32) | (uint32_t)~i;
+          if (o < last && o > best) best = o;
+        });
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+          const unsigned long long o = __shfl_xor(best, off);
+          best = o > best ? o : best;
+        }
+        __syncthreads();
+        if (lane == 0) sh.best[tid >> 6] = best;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+        if (best == 0) break;
+        last = best;
+        if (tid == 0) emit(done, (uint32_t)(best >> 32), (int)~(uint32_t)best);
+      }
+    }
+  }
+  for (int j = done + tid; j < k; j += NT) emit(j, 0u, -1);
+}
+
+// One workgroup per row (or per part of a row): every element is read once, kUnroll 16-byte slots in flight per thread.
+template <int DT, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
+  constexpr int NT = kRowThreads, VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
+  __shared__ BlockRed<NT> red;
+  __shared__ int holder;
+  __shared__ typename std::conditional<TOP, TopShared<DT>, int>::type top_sh;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x - (int)(row * a.parts);
+  const bool seen = row_seen(a.r, row);
+  if (!seen && !ENT && !TOP) {
+    if (tid == 0 && part == 0 && a.log_prob) a.log_prob[row] = 0.f;
+    return;
+  }
+  const int n = row_size(a.r, row), V = a.r.V;
+  const int ns = (n + VEC - 1) / VEC;
+  // parts are whole rounds of NT slots, so that their accesses stay contiguous
+  const int rounds = (ns + NT - 1) / NT, per = ((rounds + a.parts - 1) / a.parts) * NT;
+  const int s0 = part * per < ns ? part * per : ns, s1 = s0 + per < ns ? s0 + per : ns;
+  const char* p = a.r.x + row * a.r.ld * ES;
+  int gsz = (s1 - s0 + NT * kGroups - 1) / (NT * kGroups);    // slots per group of the selection
+  gsz = gsz < kUnroll ? kUnroll : (gsz + kUnroll - 1) / kUnroll * kUnroll;
+  Online on;
+  float gmx = -INFINITY;
+  int in_group = 0, group = 0;
+  for (int s = s0 + tid; s < s1; s += NT * kUnroll) {
+    float v[kUnroll * VEC];
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q) {
+      const int sq = s + q * NT;
+      const int b = slot_base<VEC>(sq < s1 ? sq : s, V);
+      slot_load<DT, VEC>(p, b, v + q * VEC);
+    }
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q) {
+      const int sq = s + q * NT;
+      if (sq * VEC + VEC > n || sq >= s1) {       // the row's last slot, and past the end
+        const int b = slot_base<VEC>(sq < s1 ? sq : s, V);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (sq >= s1 || b + e < sq * VEC || b + e >= n) v[q * VEC + e] = -INFINITY;
+      }
+    }
+    if constexpr (TOP) {
+      gmx = max_of<kUnroll * VEC>(v, gmx);
+      in_group += kUnroll;
+      if (in_group == gsz) {
+        top_sh.gm[group++][tid] = gmx;
+        gmx = -INFINITY;
+        in_group = 0;
+      }
+    }
+    on.template add<kUnroll * VEC, ENT>(v, a.c);
+  }
+  if constexpr (TOP) {
+    const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
+    for (; group < groups; ++group) {
+      top_sh.gm[group][tid] = gmx;
+      gmx = -INFINITY;
+    }
+  }
+  float m, r, u;
+  block_join<NT, ENT>(on, a.c, red, &holder, m, r, u, [&](int h, float ref) {
+    float sum = 0.f;
+    for (int s = s0 + h + NT * tid; s < s1; s += NT * NT) {
+      float v[VEC];
+      const int b = slot_base<VEC>(s, V);
+      slot_load<DT, VEC>(p, b, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (b + e >= s * VEC && b + e < n && v[e] < ref) sum += exp2_hw((v[e] - ref) * a.c);
+    }
+    return sum;
+  });
+  const bool empty = m == -INFINITY && r == -1.f;
+  if (a.part) {
+    if (tid == 0) a.part[row * a.parts + part] = f32x4{m, r, u, 0.f};
+    if constexpr (TOP) {
+      uint2* o = a.part_top + (row * a.parts + part) * a.top;
+      block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, on.m,
+                         [&](int rank, uint32_t key, int i) { o[rank] = make_uint2(key, (uint32_t)i); });
+    }
+    return;
+  }
+  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
+  if (tid == 0) {
+    if (a.log_prob) {
+      float lp = 0.f;
+      if (seen) {
+        const int64_t X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
+        lp = (X < 0 || X >= n) ? NAN : (empty ? -INFINITY : (Elem<DT>::load(p, X) - m) - logs);
+      }
+      a.log_prob[row] = lp;
+    }
+    if (a.entropy) a.entropy[row] = H;
+    if (a.stats) a.stats[row] = f32x4{m, inv_s, logs, H};
+  }
+  if constexpr (TOP) {
+    if (logs != logs) {
+      for (int j = tid; j < a.top; j += NT) {
+        a.top_idx[row * a.top + j] = -1;
+        a.top_lp[row * a.top + j] = NAN;
+      }
+      return;
+    }
+    block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, on.m, [&](int rank, uint32_t key, int i) {
+      a.top_idx[row * a.top + rank] = i;
+      a.top_lp[row * a.top + rank] = i < 0 ? -INFINITY : (key_value(key) - m) - logs;
+    });
+  }
+}
+
+// (m, r, u) of a row from its parts (one wavefront, a lane per part)
+__device__ __forceinline__ void join_parts(const f32x4* part, int parts, float c, float& m, float& r, float& u) {
+  const int lane = threadIdx.x & 63;
+  const f32x4 me = lane < parts ? part[lane] : f32x4{-INFINITY, -1.f, 0.f, 0.f};
+  m = gmax<64>(me[0]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float shift = fmaxf((me[0] - ref) * c, kClampD), f = exp2_hw(shift);
+  const bool holds = me[0] == m && m != -INFINITY;
+  float a = holds ? me[1] : f * (1.f + me[1]);
+  const float b = f * (me[2] - (1.f + me[1]) * shift);
+  r = gsum<64>(a) + (gsum<64>(holds ? 1.f : 0.f) - 1.f);
+  u = gsum<64>(b);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(64) k_cat_fwd_join(Fwd a) {
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const bool seen = row_seen(a.r, row);
+  if (!seen && !a.entropy && !a.top) return;        // the parts' launch has written it
+  const int n = row_size(a.r, row);
+  const char* p = a.r.x + row * a.r.ld * (int64_t)sizeof(typename Elem<DT>::type);
+  float m, r, u;
+  join_parts(a.part + row * a.parts, a.parts, a.c, m, r, u);
+  const bool empty = m == -INFINITY && !(r != r);
+  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
+  if (lane == 0) {
+    if (a.log_prob) {
+      float lp = 0.f;
+      if (seen) {
+        const int64_t X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
+        lp = (X < 0 || X >= n) ? NAN : (empty ? -INFINITY : (Elem<DT>::load(p, X) - m) - logs);
+      }
+      a.log_prob[row] = lp;
+    }
+    if (a.entropy) a.entropy[row] = H;
+    if (a.stats) a.stats[row] = f32x4{m, inv_s, logs, H};
+  }
+  if (!a.top) return;
+  const bool bad = logs != logs;
+  // merge of the parts' ordered lists: lane = part, its head against the others'
+  const uint2* list = a.part_top + (row * a.parts + lane) * (int64_t)a.top;
+  int head = 0;
+  uint2 cur = lane < a.parts ? list[0] : make_uint2(0u, 0u);
+  for (int t = 0; t < a.top; ++t) {
+    const uint32_t top = gmax_u<64>(cur.x);
+    const uint32_t low = ~gmax_u<64>((cur.x == top) ? ~cur.y : 0u);
+    if (top != 0u && cur.x == top && cur.y == low) {
+      ++head;
+      cur = head < a.top ? list[head] : make_uint2(0u, 0u);
+    }
+    if (lane == 0) {
+      const bool none = top == 0u || bad;
+      a.top_idx[row * a.top + t] = none ? -1 : (int64_t)low;
+      a.top_lp[row * a.top + t] = bad ? NAN : (none ? -INFINITY : (key_value(top) - m) - logs);
+    }
+  }
+}
+
+// A slot of a chunk: the last slot of a row overlaps the one before it, which may be another workgroup's, so only its own
+// elements are written.
+template <int DT>
+__device__ __forceinline__ void chunk_store(char* out, int s, int base, const float* o) {
+  constexpr int VEC = Elem<DT>::N;
+  if (base == s * VEC) {
+    slot_store<DT, VEC>(out, base, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (base + e >= s * VEC) Elem<DT>::store(out, base + e, o[e]);
+  }
+}
+
+// Gradient of long rows: a workgroup per chunk of a row (kChunkSlots slots), the row's statistics are known.
+constexpr int kChunkSlots = kRowThreads * kUnroll;
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) k_cat_bwd_chunk(Bwd a) {
+  constexpr int NT = kRowThreads, VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.chunks;
+  const int s0 = (blockIdx.x - (int)(row * a.chunks)) * kChunkSlots;
+  const int n = row_size(a.r, row), V = a.r.V;
+  const int ns = (V + VEC - 1) / VEC;
+  int64_t X;
+  float gl;
+  const RowGrad g = row_grad<64>(a, row, tid & 63, n, X, gl);
+  const bool live = (g.S != 0.f || g.gh != 0.f || a.g_top) && g.inv_s != 0.f;
+  const char* p = a.r.x + row * a.r.ld * ES;
+  char* out = (char*)a.d + row * a.ld_d * ES;
+  float v[kUnroll][VEC];
+  if (live) {
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q) {
+      const int s = s0 + tid + q * NT;
+      slot_load<DT, VEC>(p, slot_base<VEC>(s < ns ? s : ns - 1, V), v[q]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kUnroll; ++q) {
+    const int s = s0 + tid + q * NT;
+    if (s >= ns) break;
+    const int b = slot_base<VEC>(s, V);
+    float o[VEC];
+    if (live) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = g.dense(v[q][e]);
+      if (b + VEC > n) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (b + e >= n) o[e] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = 0.f;
+    }
+    chunk_store<DT>(out, s, b, o);
+  }
+  if (!live) return;
+  __syncthreads();          // the dense part before the few categories written again
+  const int64_t lo = (int64_t)s0 * VEC, hi = lo + (int64_t)kChunkSlots * VEC;
+  const int entries = 1 + (a.g_top ? a.top : 0);
+  for (int j = tid; j < entries; j += NT) {
+    const int64_t v0 = j == 0 ? X : a.top_idx[row * a.top + j - 1];
+    if (v0 < lo || v0 >= hi || v0 >= n) continue;
+    Elem<DT>::store(out, v0, g.at(Elem<DT>::load(p, v0), own_share(a, row, v0, X, gl)));
+  }
+}
+
+
+// The teacher's distribution over one row by a workgroup, entry j on thread j (k <= NT): p and log p of this thread's entry
+// (p = 0 where it does not count), its index (-1), and what holds for the row.
+struct TeacherEntry {
+  float p, lp;
+  int i;
+  bool any, bad;
+};
+template <int NT>
+__device__ __forceinline__ TeacherEntry teacher_row(const Teacher& t, int64_t row, int64_t rows, int n, BlockRed<NT>& red) {
+  static_assert(NT >= kMaxTeacher, "one entry per thread");
+  TeacherEntry e{0.f, 0.f, -1, false, false};
+  float x = -INFINITY;
+  bool bad = false;
+  if ((int)threadIdx.x < t.k) {
+    const int64_t at = wrap(row, t.t_period, rows) * t.k + threadIdx.x;
+    const int64_t i = t.idx[at];
+    const float v = teacher_logit(t, at);
+    if (entry_counts(v, i)) {
+      bad = i >= n || !(v < INFINITY);
+      x = bad ? -INFINITY : v;
+      e.i = bad ? -1 : (int)i;
+    }
+  }
+  const float tm = block_max<NT>(x, red);
+  const bool counts = e.i >= 0;
+  float s = counts && x < tm ? exp2_hw((x - tm) * t.c) : 0.f, held = counts && x == tm ? 1.f : 0.f, b = bad ? 1.f : 0.f;
+  block_sum3<NT>(s, held, b, red);
+  e.bad = b > 0.f;
+  e.any = held > 0.f || e.bad;
+  if (counts) {
+    e.lp = (x - tm) * t.inv_T - log1pf(s + (held - 1.f));
+    e.p = expf(e.lp);
+  }
+  return e;
+}
+
+struct SparseShared {
+  float p[kMaxTeacher];
+  int i[kMaxTeacher];
+};
+// all of the teacher's probability on category i (it may be given more than once): the same sum for each of its entries
+__device__ __forceinline__ float share_of(const SparseShared& sh, int k, int i) {
+  float p = 0.f;
+  for (int j = 0; j < k; ++j) p += sh.i[j] == i ? sh.p[j] : 0.f;
+  return p;
+}
+
+// The values of a packed slot for one pass over the row.  The compiler is made to forget what it knows of them and to keep
+// the slots in order: it would otherwise hold the unpacked values, twice the registers, across the passes.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int DT>
+__device__ __forceinline__ void pass_over(u32x4& r, float* v) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" : "+v"(r));
+  Elem<DT>::unpack(__builtin_bit_cast(Raw16, r), v);
+}
+__device__ __forceinline__ int again(int t) {
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// Loss and gradient of a row that fits the registers of one workgroup (NV slots per thread): the row is read once.
+template <int DT, int NT, int NV>
+__global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
+  constexpr int VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
+  __shared__ BlockRed<NT> red;
+  __shared__ SparseShared sp;
+  __shared__ int holder;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int V = a.r.V, ns = (V + VEC - 1) / VEC;
+  char* out = (char*)a.d + row * a.ld_d * ES;
+  const float w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
+  auto zeros = [&]() {
+    const float z[VEC] = {};
+    for (int s = tid; s < ns; s += NT) slot_store<DT, VEC>(out, slot_base<VEC>(s, V), z);
+  };
+  if (w == 0.f) {
+    if (tid == 0) {
+      if (a.per_row) a.per_row[row] = 0.f;
+      a.loss_part[row] = 0.0;
+    }
+    if (a.d) zeros();
+    return;
+  }
+  const char* p = a.r.x + row * a.r.ld * ES;
+  u32x4 raw[NV];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const int s = tid + NT * q;
+    raw[q] = __builtin_bit_cast(u32x4, *(const Raw16*)(p + (uint32_t)(slot_base<VEC>(s < ns ? s : ns - 1, V) * ES)));
+  }
+  const int n = row_size(a.r, row);
+  const TeacherEntry te = teacher_row<NT>(a.t, row, a.r.rows, n, red);
+  const float xi = te.i >= 0 ? Elem<DT>::load(p, te.i) : 0.f;
+  // what does not count becomes -inf, once: past the row's size, and what a last slot shares with the one before it
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    if (NT * (q + 1) * VEC <= n) continue;
+    const int s = again(tid) + NT * q;
+    if (s * VEC + VEC > n) {
+      const int b = slot_base<VEC>(s < ns ? s : ns - 1, V);
+      float v[VEC];
+      pass_over<DT>(raw[q], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (b + e < s * VEC || b + e >= n) v[e] = -INFINITY;
+      Raw16 w;
+      Elem<DT>::pack(v, w);
+      raw[q] = __builtin_bit_cast(u32x4, w);
+    }
+  }
+  Online on;
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    float v[VEC];
+    pass_over<DT>(raw[q], v);
+    on.m = max_of<VEC>(v, on.m);
+  }
+  const float local = on.m == -INFINITY ? 0.f : on.m;
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    float v[VEC];
+    pass_over<DT>(raw[q], v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) on.s += exp2_hw((v[e] - local) * a.t.c);
+  }
+  asm volatile("" : "+v"(on.s));        // summed here, not where it is used
+  float m, r, u;
+  block_join<NT, false>(on, a.t.c, red, &holder, m, r, u, [&](int h, float ref) {
+    float sum = 0.f;
+    if (h == tid) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        float v[VEC];
+        pass_over<DT>(raw[q], v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += v[e] < ref ? exp2_hw((v[e] - ref) * a.t.c) : 0.f;
+      }
+    }
+    return sum;
+  });
+  const bool empty = m == -INFINITY && r == -1.f;
+  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float lq = (xi - m) * a.t.inv_T - logs;
+  float kl = (te.i >= 0 && te.p > 0.f && !empty) ? te.p * (te.lp - lq) : 0.f, z0 = 0.f, z1 = 0.f;
+  if (tid < a.t.k) {
+    sp.p[tid] = te.p;
+    sp.i[tid] = te.i;
+  }
+  block_sum3<NT>(kl, z0, z1, red);
+  if (te.any && empty) kl = INFINITY;
+  if (te.bad) kl = NAN;
+  if (tid == 0) {
+    if (a.per_row) a.per_row[row] = kl;
+    if (a.stats) a.stats[row] = f32x4{m, inv_s, logs, 0.f};
+    a.loss_part[row] = (double)w * (double)kl;
+  }
+  if (!a.d) return;
+  if (!te.any || empty) {
+    zeros();
+    return;
+  }
+  const float scale = te.bad ? NAN : w * a.t.inv_T, f = scale * inv_s;
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const int s = again(tid) + NT * q;
+    if (s >= ns) break;
+    float v[VEC];
+    pass_over<DT>(raw[q], v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = exp2_hw((v[e] - m) * a.t.c) * f;
+    if (s * VEC + VEC <= V) slot_store<DT, VEC>(out, s * VEC, v);
+    else chunk_store<DT>(out, s, V - VEC, v);
+  }
+  __syncthreads();          // the dense part before the teacher's categories are written again
+  if (te.i >= 0 && !te.bad) Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te.i)));
+}
+
+// Rows that are read by several workgroups: their parts' statistics (k_cat_fwd_row) joined, and the loss.
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) k_cat_distill_join(Dist a) {
+  constexpr int NT = kRowThreads, ES = sizeof(typename Elem<DT>::type);
+  __shared__ BlockRed<NT> red;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const float w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
+  if (w == 0.f) {
+    if (tid == 0) {
+      if (a.per_row) a.per_row[row] = 0.f;
+      a.loss_part[row] = 0.0;
+    }
+    return;
+  }
+  const int n = row_size(a.r, row);
+  const char* p = a.r.x + row * a.r.ld * ES;
+  const TeacherEntry te = teacher_row<NT>(a.t, row, a.r.rows, n, red);
+  const float xi = te.i >= 0 ? Elem<DT>::load(p, te.i) : 0.f;
+  float m, r, u;
+  join_parts(a.part + row * a.parts, a.parts, a.t.c, m, r, u);     // every wavefront does the same
+  const bool empty = m == -INFINITY && !(r != r);
+  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  float kl = (te.i >= 0 && te.p > 0.f && !empty) ? te.p * (te.lp - ((xi - m) * a.t.inv_T - logs)) : 0.f, z0 = 0.f, z1 = 0.f;
+  block_sum3<NT>(kl, z0, z1, red);
+  if (te.any && empty) kl = INFINITY;
+  if (te.bad) kl = NAN;
+  if (tid == 0) {
+    if (a.per_row) a.per_row[row] = kl;
+    a.stats[row] = f32x4{m, inv_s, logs, 0.f};
+    a.loss_part[row] = (double)w * (double)kl;
+  }
+}
+
+// The gradient of rows whose statistics are known, a workgroup per chunk of a row at a time.
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) k_cat_distill_chunk(Dist a) {
+  constexpr int NT = kRowThreads, VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
+  __shared__ BlockRed<NT> red;
+  __shared__ SparseShared sp;
+  const float gs = a.gscale ? *a.gscale : 1.f;
+  if (a.unless_one && gs == 1.f) return;
+  const int tid = threadIdx.x;
+  const int V = a.r.V, ns = (V + VEC - 1) / VEC;
+  const int64_t items = a.r.rows * a.chunks;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = item / a.chunks;
+    const int s0 = (int)(item - row * a.chunks) * kChunkSlots;
+    const int n = row_size(a.r, row);
+    const char* p = a.r.x + row * a.r.ld * ES;
+    char* out = (char*)a.d + row * a.ld_d * ES;
+    const float w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
+    bool live = w != 0.f;
+    float v[kUnroll][VEC];
+    TeacherEntry te{0.f, 0.f, -1, false, false};
+    f32x4 st = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const int s = s0 + tid + q * NT;
+        slot_load<DT, VEC>(p, slot_base<VEC>(s < ns ? s : ns - 1, V), v[q]);
+      }
+      st = a.stats[row];
+      te = teacher_row<NT>(a.t, row, a.r.rows, n, red);
+      if (tid < a.t.k) {
+        sp.p[tid] = te.p;
+        sp.i[tid] = te.i;
+      }
+      live = te.any && st[1] != 0.f;
+    }
+    const float scale = te.bad ? NAN : gs * w * a.t.inv_T, f = scale * st[1];
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q) {
+      const int s = s0 + tid + q * NT;
+      if (s < ns) {
+        const int b = slot_base<VEC>(s, V);
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = live && b + e < n ? exp2_hw((v[q][e] - st[0]) * a.t.c) * f : 0.f;
+        chunk_store<DT>(out, s, b, o);
+      }
+    }
+    __syncthreads();        // the dense part, and sp, before the teacher's categories are written again
+    const int64_t lo = (int64_t)s0 * VEC;
+    if (live && !te.bad && te.i >= lo && te.i < lo + (int64_t)kChunkSlots * VEC) {
+      const float lq = (Elem<DT>::load(p, te.i) - st[0]) * a.t.inv_T - st[2];
+      Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te.i)));
+    }
+    __syncthreads();        // sp is free again
+  }
+}
+
+// The loss: the workgroups' (or rows') shares summed in a fixed order.
+constexpr int kLossThreads = 1024;
+__global__ void __launch_bounds__(kLossThreads) k_cat_loss(const double* part, int64_t n, float* loss) {
+  __shared__ double w[kLossThreads / 64];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += kLossThreads) s += part[i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < kLossThreads / 64; ++i) t += w[i];
+    *loss = (float)t;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host side
+constexpr int64_t kMaxGrid = 0x7fffffffll;
+constexpr int kSmallMax = DMV_CAT_SHORT_ROW;   // longest row of the register kernels of short rows
+constexpr int kMaxParts = 64;           // a join's lane per part
+
+int check_rows(const DmvCatRows* r) {
+  if (!r || r->rows < 0 || r->V < 1 || r->ld < 0) return DMV_E_BADARG;
+  if (r->dtype < DMV_F32 || r->dtype > DMV_F16) return DMV_E_UNSUPPORTED;
+  if (r->rows == 0) return DMV_OK;
+  if (!r->logits || ((uintptr_t)r->logits % elem_size(r->dtype)) != 0) return DMV_E_BADARG;
+  if ((r->X && r->x_period < 1) || (r->M && r->m_period < 1) || (r->sizes && r->size_period < 1)) return DMV_E_BADARG;
+  // a workgroup per row and part, and slot numbers in 32 bits with room for a chunk
+  if (r->rows > kMaxGrid / kMaxParts || r->V > 0x7fffffff - (1 << 20)) return DMV_E_UNSUPPORTED;
+  return DMV_OK;
+}
+Rows rows_of(const DmvCatRows* r) {
+  return Rows{(const char*)r->logits, r->ld, r->rows, r->V, r->X, r->M, r->sizes, r->x_period, r->m_period, r->size_period};
+}
+
+// Short rows: `f` gets the tag of the smallest register tile that holds V elements (16 elements a lane; rows shorter
+// than a 16-byte slot are read one element at a time).
+template <int DT_, int VEC_, int L_, int SL_>
+struct Tile {
+  static constexpr int DT = DT_, VEC = VEC_, L = L_, SL = SL_;
+};
+template <int DT, typename F>
+void small_tile(int V, F f) {
+  constexpr int N = Elem<DT>::N, S = 16 / N;
+  const int ns = (V + N - 1) / N;
+  if (V < N) return f(Tile<DT, 1, 4, 2>());
+  if (ns <= 4) return f(Tile<DT, N, 4, 1>());
+  if (ns <= 8) return f(Tile<DT, N, 4, 2>());
+  if constexpr (S == 4)
+    if (ns <= 16) return f(Tile<DT, N, 4, 4>());
+  if (ns <= 8 * S) return f(Tile<DT, N, 8, S>());
+  if (ns <= 16 * S) return f(Tile<DT, N, 16, S>());
+  if (ns <= 32 * S) return f(Tile<DT, N, 32, S>());
+  return f(Tile<DT, N, 64, S>());
+}
+template <typename F>
+void by_type(int dt, F f) {
+  if (dt == DMV_F32) f(std::integral_constant<int, DMV_F32>());
+  else if (dt == DMV_BF16) f(std::integral_constant<int, DMV_BF16>());
+  else f(std::integral_constant<int, DMV_F16>());
+}
+
+// Workgroups per long row: enough to occupy the chip, but at least one full round of loads (kUnroll slots per thread) each.
+int parts_of(int64_t rows, int V, int dt) {
+  const int64_t rounds = ((int64_t)V + (int64_t)kChunkSlots * vec_elems(dt) - 1) / ((int64_t)kChunkSlots * vec_elems(dt));
+  int64_t parts = (1024 + rows - 1) / rows;
+  if (parts > rounds) parts = rounds;
+  if (parts > kMaxParts) parts = kMaxParts;
+  return parts < 1 ? 1 : (int)parts;
+}
+// slots per thread of the kernel that keeps a row in a workgroup's registers; 0: it does not fit
+constexpr int64_t kRowMinRows = 128;    // fewer rows: several workgroups per row
+int64_t row_slots(int V, int dt) { return ((int64_t)V + vec_elems(dt) - 1) / vec_elems(dt); }
+bool row_fits(int64_t rows, int V, int dt) { return rows >= kRowMinRows && row_slots(V, dt) <= 16 * 1024; }
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+template <int DT>
+void launch_fwd_rows(const Fwd& a, bool entropy, hipStream_t st) {
+  const dim3 grid((unsigned)(a.r.rows * a.parts)), block(kRowThreads);
+  if (a.top) {
+    if (entropy) k_cat_fwd_row<DT, true, true><<<grid, block, 0, st>>>(a);
+    else k_cat_fwd_row<DT, false, true><<<grid, block, 0, st>>>(a);
+  } else {
+    if (entropy) k_cat_fwd_row<DT, true, false><<<grid, block, 0, st>>>(a);
+    else k_cat_fwd_row<DT, false, false><<<grid, block, 0, st>>>(a);
+  }
+}
+
+template <int DT>
+void launch_distill_row(const Dist& a, hipStream_t st) {
+  const int64_t ns = row_slots(a.r.V, DT);
+  const dim3 grid((unsigned)a.r.rows);
+  if (ns <= 2 * 256) k_cat_distill_row<DT, 256, 2><<<grid, 256, 0, st>>>(a);
+  else if (ns <= 4 * 256) k_cat_distill_row<DT, 256, 4><<<grid, 256, 0, st>>>(a);
+  else if (ns <= 8 * 256) k_cat_distill_row<DT, 256, 8><<<grid, 256, 0, st>>>(a);
+  else if (ns <= 8 * 512) k_cat_distill_row<DT, 512, 8><<<grid, 512, 0, st>>>(a);
+  else if (ns <= 8 * 1024) k_cat_distill_row<DT, 1024, 8><<<grid, 1024, 0, st>>>(a);
+  else k_cat_distill_row<DT, 1024, 16><<<grid, 1024, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" size_t dmv_cat_log_prob_ws_bytes(const DmvCatRows* r, int32_t top) {
+  if (check_rows(r) != DMV_OK || r->rows == 0 || top < 0 || top > kMaxTop || r->V <= kSmallMax) return 0;
+  const int parts = parts_of(r->rows, r->V, r->dtype);
+  if (parts == 1) return 0;
+  return (size_t)r->rows * parts * (sizeof(f32x4) + (size_t)top * sizeof(uint2));
+}
+
+extern "C" int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* entropy, int32_t top, float* top_log_prob,
+                                int64_t* top_index, float* stats, void* ws, size_t ws_bytes, void* stream) {
+  const int rc = check_rows(r);
+  if (rc != DMV_OK) return rc;
+  if (top < 0) return DMV_E_BADARG;
+  if (top > kMaxTop) return DMV_E_UNSUPPORTED;
+  if (r->rows == 0) return DMV_OK;
+  if ((log_prob && !r->X) || (!log_prob && !entropy && !top) || (top && (!top_log_prob || !top_index))) return DMV_E_BADARG;
+  if (((uintptr_t)stats & 15) != 0 || ((uintptr_t)ws & 15) != 0) return DMV_E_BADARG;
+  Fwd a{rows_of(r), log_prob, entropy, top, top_log_prob, top_index, (f32x4*)stats, kLog2e, 1, nullptr, nullptr};
+  hipStream_t st = (hipStream_t)stream;
+  if (r->V <= kSmallMax) {
+    by_type(r->dtype, [&](auto dt) {
+      small_tile<decltype(dt)::value>(r->V, [&](auto t) {
+        typedef decltype(t) T;
+        k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL>
+            <<<dmv_ceil_div(r->rows, kSmallThreads / T::L), kSmallThreads, 0, st>>>(a);
+      });
+    });
+    DMV_HIP_CHECK_LAUNCH();
+    return DMV_OK;
+  }
+  a.parts = parts_of(r->rows, r->V, r->dtype);
+  if (a.parts > 1) {
+    if (!ws || ws_bytes < dmv_cat_log_prob_ws_bytes(r, top)) return DMV_E_WORKSPACE;
+    a.part = (f32x4*)ws;
+    a.part_top = (uint2*)(a.part + r->rows * a.parts);
+  }
+  by_type(r->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    launch_fwd_rows<DT>(a, entropy != nullptr, st);
+    if (a.parts > 1) k_cat_fwd_join<DT><<<(unsigned)r->rows, 64, 0, st>>>(a);
+  });
+  DMV_HIP_CHECK_LAUNCH();
+  return DMV_OK;
+}
+
+extern "C" int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats, const float* g_log_prob, const float* g_entropy,
+                                         int32_t top, const int64_t* top_index, const float* g_top, void* d_logits, int64_t ld_d,
+                                         void* stream) {
+  const int rc = check_rows(r);
+  if (rc != DMV_OK) return rc;
+  if (top < 0) return DMV_E_BADARG;
+  if (top > kMaxTop) return DMV_E_UNSUPPORTED;
+  if (r->rows == 0) return DMV_OK;
+  if ((g_log_prob && !r->X) || (g_top && (!top || !top_index)) || ld_d < r->V) return DMV_E_BADARG;
+  if (!stats || ((uintptr_t)stats & 15) != 0 || !d_logits || ((uintptr_t)d_logits % elem_size(r->dtype)) != 0) return DMV_E_BADARG;
+  Bwd a{rows_of(r), (const f32x4*)stats, g_log_prob, g_entropy, top, top_index, g_top, d_logits, ld_d, 1};
+  hipStream_t st = (hipStream_t)stream;
+  if (r->V <= kSmallMax) {
+    by_type(r->dtype, [&](auto dt) {
+      small_tile<decltype(dt)::value>(r->V, [&](auto t) {
+        typedef decltype(t) T;
+        k_cat_bwd_small<T::DT, T::VEC, T::L, T::SL>
+            <<<dmv_ceil_div(r->rows, kSmallThreads / T::L), kSmallThreads, 0, st>>>(a);
+      });
+    });
+    DMV_HIP_CHECK_LAUNCH();
+    return DMV_OK;
+  }
+  a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
+  if (r->rows > kMaxGrid / a.chunks) return DMV_E_UNSUPPORTED;
+  by_type(r->dtype, [&](auto dt) {
+    k_cat_bwd_chunk<decltype(dt)::value><<<(unsigned)(r->rows * a.chunks), kRowThreads, 0, st>>>(a);
+  });
+  DMV_HIP_CHECK_LAUNCH();
+  return DMV_OK;
+}
+
+static int check_teacher(const DmvCatRows* r, const DmvCatTeacher* t) {
+  if (!t || t->k < 1 || !t->logits || !t->index || t->period < 1 || (t->weight && t->w_period < 1)) return DMV_E_BADARG;
+  if (t->dtype < DMV_F32 || t->dtype > DMV_F16 || t->k > kMaxTeacher) return DMV_E_UNSUPPORTED;
+  if (((uintptr_t)t->logits % elem_size(t->dtype)) != 0 || !(t->temperature > 0.f) || !(t->temperature <= 3.4e38f)) return DMV_E_BADARG;
+  return DMV_OK;
+}
+static Dist dist_of(const DmvCatRows* r, const DmvCatTeacher* t) {
+  Dist a{};
+  a.r = rows_of(r);
+  a.t = Teacher{t->logits, t->index, t->weight, t->period, t->w_period, t->k, t->dtype, kLog2e / t->temperature, 1.f / t->temperature};
+  a.chunks = a.parts = 1;
+  return a;
+}
+static int64_t loss_parts(const DmvCatRows* r) {
+  int64_t n = r->rows;
+  if (r->V <= kSmallMax)
+    by_type(r->dtype, [&](auto dt) {
+      small_tile<decltype(dt)::value>(r->V, [&](auto t) { n = dmv_ceil_div(r->rows, kSmallThreads / decltype(t)::L); });
+    });
+  return n;
+}
+
+extern "C" size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r) {
+  if (check_rows(r) != DMV_OK || r->rows == 0) return 0;
+  size_t n = up16((size_t)loss_parts(r) * sizeof(double));
+  if (r->V > kSmallMax && !row_fits(r->rows, r->V, r->dtype))
+    n += (size_t)r->rows * (1 + parts_of(r->rows, r->V, r->dtype)) * sizeof(f32x4);
+  return n;
+}
+
+extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, float* per_row, float* loss, float* stats, void* d_logits,
+                               int64_t ld_d, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_rows(r);
+  if (rc != DMV_OK) return rc;
+  if (!loss || (d_logits && ld_d < r->V)) return DMV_E_BADARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (r->rows == 0) {
+    k_cat_loss<<<1, kLossThreads, 0, st>>>(nullptr, 0, loss);
+    DMV_HIP_CHECK_LAUNCH();
+    return DMV_OK;
+  }
+  rc = check_teacher(r, t);
+  if (rc != DMV_OK) return rc;
+  if (((uintptr_t)stats & 15) != 0 || (d_logits && ((uintptr_t)d_logits % elem_size(r->dtype)) != 0)) return DMV_E_BADARG;
+  if (!ws || ((uintptr_t)ws & 15) != 0 || ws_bytes < dmv_cat_distill_ws_bytes(r)) return DMV_E_WORKSPACE;
+  const int64_t n_loss = loss_parts(r);
+  Dist a = dist_of(r, t);
+  a.per_row = per_row;
+  a.loss_part = (double*)ws;
+  a.stats = (f32x4*)stats;
+  a.d = d_logits;
+  a.ld_d = ld_d;
+  if (r->V <= kSmallMax) {
+    by_type(r->dtype, [&](auto dt) {
+      small_tile<decltype(dt)::value>(r->V, [&](auto tile) {
+        typedef decltype(tile) T;
+        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)n_loss, kSmallThreads, 0, st>>>(a);
+      });
+    });
+  } else if (row_fits(r->rows, r->V, r->dtype)) {
+    by_type(r->dtype, [&](auto dt) { launch_distill_row<decltype(dt)::value>(a, st); });
+  } else {
+    a.parts = parts_of(r->rows, r->V, r->dtype);
+    f32x4* own = (f32x4*)((char*)ws + up16((size_t)n_loss * sizeof(double)));
+    if (!a.stats) a.stats = own;
+    a.part = own + r->rows;
+    a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
+    Fwd f{a.r, nullptr, nullptr, 0, nullptr, nullptr, nullptr, a.t.c, a.parts, a.part, nullptr};
+    const int64_t items = r->rows * a.chunks;
+    by_type(r->dtype, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      k_cat_fwd_row<DT, false, false><<<(unsigned)(r->rows * a.parts), kRowThreads, 0, st>>>(f);
+      k_cat_distill_join<DT><<<(unsigned)r->rows, kRowThreads, 0, st>>>(a);
+      if (a.d) k_cat_distill_chunk<DT><<<(unsigned)(items < 8192 ? items : 8192), kRowThreads, 0, st>>>(a);
+    });
+  }
+  k_cat_loss<<<1, kLossThreads, 0, st>>>(a.loss_part, n_loss, loss);
+  DMV_HIP_CHECK_LAUNCH();
+  return DMV_OK;
+}
+
+extern "C" int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher* t, const float* gscale, int32_t unless_one,
+                                        const float* stats, void* d_logits, int64_t ld_d, void* stream) {
+  int rc = check_rows(r);
+  if (rc != DMV_OK) return rc;
+  if (ld_d < r->V || !gscale) return DMV_E_BADARG;
+  if (r->rows == 0) return DMV_OK;
+  rc = check_teacher(r, t);
+  if (rc != DMV_OK) return rc;
+  if (!d_logits || ((uintptr_t)d_logits % elem_size(r->dtype)) != 0) return DMV_E_BADARG;
+  if (r->V > kSmallMax && (!stats || ((uintptr_t)stats & 15) != 0)) return DMV_E_BADARG;
+  Dist a = dist_of(r, t);
+  a.gscale = gscale;
+  a.unless_one = unless_one;
+  a.stats = r->V > kSmallMax ? (f32x4*)const_cast<float*>(stats) : nullptr;   // short rows form theirs again
+  a.d = d_logits;
+  a.ld_d = ld_d;
+  hipStream_t st = (hipStream_t)stream;
+  by_type(r->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (r->V <= kSmallMax) {
+      small_tile<DT>(r->V, [&](auto tile) {
+        typedef decltype(tile) T;
+        const int64_t groups = (r->rows + kSmallThreads / T::L - 1) / (kSmallThreads / T::L);
+        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)groups, kSmallThreads, 0, st>>>(a);
+      });
+    } else {
+      a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
+      const int64_t items = r->rows * a.chunks;
+      k_cat_distill_chunk<DT><<<(unsigned)(items < 2048 ? items : 2048), kRowThreads, 0, st>>>(a);
+    }
+  });
+  DMV_HIP_CHECK_LAUNCH();
+  return DMV_OK;
+}

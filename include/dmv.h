@@ -509,6 +509,77 @@ int dmv_grid_divergences(int32_t gen_dist, int32_t D, int32_t Zd, int64_t Nz, co
                          const float* log_marg, int32_t Kq, const float* q_mu, const float* q_sigma, float* out,
                          void* stream);
 
+/* ----- categorical rows --------------------------------------------------------------------
+ * Categorical entries of incomplete data (table columns, pixels or tokens as categories), mixture and importance
+ * weights: a row is the logits of one entry over its categories.  No counterpart in the reference, whose categorical
+ * work is torch.distributions.Categorical (vgiwae/models/vae.py:113-129) and the draws above.
+ *   logits [rows][ld] of type dtype, the first V of a pitch of ld elements (ld >= 0; any element alignment).  Samples are
+ *   laid out as everywhere else, n = (s*B + b)*D + d for D categorical entries, so the per-row arrays repeat: row r
+ *   reads X[r % x_period] (the given category), M[r % m_period] (NULL: all seen; a row that is not seen has
+ *   log-probability 0 whatever X holds), sizes[r % size_period] (NULL: V; categories >= size do not exist, whatever
+ *   their logits hold; clamped to 0..V).
+ * A row without any category of non-zero probability (size 0, or all logits -inf) has entropy 0, log-probability -inf,
+ * no alternatives and a zero gradient.  NaN or +inf among a row's logits makes its outputs NaN (alternatives -1); a given
+ * category outside the row's, where it is seen, makes that row's log-probability and gradient NaN. */
+enum { DMV_F32 = 0, DMV_BF16 = 1, DMV_F16 = 2 };
+#define DMV_CAT_MAX_TOP 64
+#define DMV_CAT_MAX_TEACHER 256
+#define DMV_CAT_SHORT_ROW 1024
+typedef struct DmvCatRows {
+  const void* logits;
+  int64_t ld;
+  int64_t rows;
+  int32_t V;
+  int32_t dtype;          /* DMV_F32 / DMV_BF16 / DMV_F16 */
+  const int64_t* X;
+  int64_t x_period;
+  const uint8_t* M;
+  int64_t m_period;
+  const int32_t* sizes;
+  int64_t size_period;
+} DmvCatRows;
+
+/* log_prob [rows] = M log q_X (NULL: not wanted), entropy [rows] = -sum q log q (NULL), the `top` (0..64) most probable
+ * categories in order, the lower index first among equal logits: top_log_prob, top_index [rows][top], -inf / -1 past the
+ * categories of non-zero probability.  stats (nullable, [rows][4], 16-byte aligned): what the backward call reads; rows
+ * that are not seen have none when neither entropy nor alternatives are asked for.
+ * ws: dmv_cat_log_prob_ws_bytes bytes, 16-byte aligned (may be 0). */
+size_t dmv_cat_log_prob_ws_bytes(const DmvCatRows* r, int32_t top);
+int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* entropy, int32_t top, float* top_log_prob, int64_t* top_index,
+                     float* stats, void* ws, size_t ws_bytes, void* stream);
+/* Gradient of the same outputs: d_logits [rows][ld_d], all V columns written (zeros past a row's size), for upstream
+ * gradients g_log_prob [rows], g_entropy [rows], g_top [rows][top] (NULL: none; top_index is the forward's). */
+int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats, const float* g_log_prob, const float* g_entropy, int32_t top,
+                              const int64_t* top_index, const float* g_top, void* d_logits, int64_t ld_d, void* stream);
+
+/* Distillation from a teacher's top logits: with p = softmax(logits / T) over the k (1..256) entries given for row
+ * r % period (an entry with a negative index or a logit of -inf is empty; a category given twice counts twice) and q =
+ * softmax(row / T) over all of the row's categories,
+ *   per_row[r] = KL(p || q) = sum_j p_j (log p_j - log q_index[j]),   loss = sum_r weight[r % w_period] per_row[r]
+ * (weight NULL: 1).  Rows of weight 0 are not read and have per_row 0; rows without entries have 0.  d_logits (nullable)
+ * receives the gradient of loss: weight / T (q - p).  An index at or past the row's size, or a logit of NaN or +inf,
+ * makes the row's loss and gradient NaN; categories of probability 0 under q with p > 0 make the loss inf.  The sum of
+ * the loss has a fixed order and is held in 64 bits.
+ * stats: needed by the backward call for V > DMV_CAT_SHORT_ROW ([rows][4], 16-byte aligned), nullable.
+ * ws: dmv_cat_distill_ws_bytes bytes, 16-byte aligned. */
+typedef struct DmvCatTeacher {
+  const void* logits;     /* [period][k] */
+  const int64_t* index;   /* [period][k] */
+  int64_t period;
+  int32_t k;
+  int32_t dtype;
+  const float* weight;
+  int64_t w_period;
+  float temperature;      /* > 0 */
+} DmvCatTeacher;
+size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r);
+int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, float* per_row, float* loss, float* stats, void* d_logits,
+                    int64_t ld_d, void* ws, size_t ws_bytes, void* stream);
+/* d_logits = *gscale times the gradient of loss, from the logits again (one rounding).  unless_one: return at once, on the
+ * device, if *gscale is 1: d_logits already holds what dmv_cat_distill wrote. */
+int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher* t, const float* gscale, int32_t unless_one,
+                             const float* stats, void* d_logits, int64_t ld_d, void* stream);
+
 /* Optimiser step (vgiwae/models/vae.py:349-390: Adam / AMSGrad with one parameter group per network, preceded by
  * clip_grad_norm_ over all parameters; shared/mvb2_manual_optimisation.py:9-11).  One call =
  *   norm = || all grads ||_2;  coef = max_norm > 0 ? min(1, max_norm / (norm + 1e-6)) : 1;  g' = coef * g   (grads are

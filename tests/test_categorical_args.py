@@ -1,0 +1,156 @@
+"""What the categorical operators refuse, on the CPU: the Python entry points' checks of their arguments, and the C entry
+points' error codes (argument checks come before any launch, so none of these calls reaches a GPU)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import demiss_vae_amd as dmv
+from demiss_vae_amd import _lib as L
+
+
+def _logits(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("kw, error, what", [
+    (dict(), ValueError, "nothing asked"),
+    (dict(M=torch.ones(4, dtype=torch.bool), entropy=True), ValueError, "give X"),
+    (dict(top=-1), ValueError, "top"),
+    (dict(top=65), ValueError, "top"),
+    (dict(X=torch.zeros(4)), TypeError, "X of type"),
+    (dict(X=torch.zeros(4, dtype=torch.bool)), TypeError, "X of type"),
+    (dict(X=torch.zeros(3, dtype=torch.long)), ValueError, "does not fit"),
+    (dict(X=torch.zeros(2, 4, dtype=torch.long)), ValueError, "does not fit"),
+    (dict(X=torch.zeros(4, dtype=torch.long), M=torch.ones(4)), TypeError, "a mask"),
+    (dict(X=torch.zeros(4, dtype=torch.long), M=torch.ones(5, dtype=torch.bool)), ValueError, "does not fit"),
+    (dict(entropy=True, sizes=torch.ones(4)), TypeError, "sizes"),
+    (dict(entropy=True, sizes=torch.ones(2, dtype=torch.int32)), ValueError, "does not fit"),
+    (dict(entropy=True), RuntimeError, "no CPU path"),
+])
+def test_log_prob_refuses(kw, error, what):
+    with pytest.raises(error, match=what):
+        dmv.categorical_log_prob(_logits(4, 7), **kw)
+
+
+@pytest.mark.parametrize("logits, error", [
+    (_logits(4, 0), ValueError), (torch.zeros(4, 3, dtype=torch.int32), TypeError), (_logits(4, 3, dtype=torch.float64), TypeError),
+    (torch.tensor(1.0), ValueError), ([1.0, 2.0], ValueError)])
+def test_both_refuse_logits(logits, error):
+    with pytest.raises(error):
+        dmv.categorical_log_prob(logits, entropy=True)
+    with pytest.raises(error):
+        dmv.distill_top_logits(logits, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long))
+
+
+@pytest.mark.parametrize("top, index, kw, error, what", [
+    (torch.zeros(4, 2), torch.zeros(4, 3, dtype=torch.long), {}, ValueError, "one shape"),
+    (torch.zeros(4, 2), torch.zeros(4, 2), {}, TypeError, "top_index"),
+    (torch.zeros(4, 2, dtype=torch.float64), torch.zeros(4, 2, dtype=torch.long), {}, TypeError, "top_logits"),
+    (torch.zeros(4, 0), torch.zeros(4, 0, dtype=torch.long), {}, ValueError, "entries per row"),
+    (torch.zeros(4, 257), torch.zeros(4, 257, dtype=torch.long), {}, ValueError, "entries per row"),
+    (torch.zeros(5, 2), torch.zeros(5, 2, dtype=torch.long), {}, ValueError, "does not fit"),
+    (torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), dict(temperature=0.0), ValueError, "temperature"),
+    (torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), dict(temperature=float("nan")), ValueError, "temperature"),
+    (torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), dict(temperature=float("inf")), ValueError, "temperature"),
+    (torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), dict(weight=torch.ones(3)), ValueError, "does not fit"),
+    (torch.zeros(4, 2, requires_grad=True), torch.zeros(4, 2, dtype=torch.long), {}, ValueError, "detach"),
+    (torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), dict(weight=torch.ones(4, requires_grad=True)), ValueError, "detach"),
+    (torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), {}, RuntimeError, "no CPU path"),
+])
+def test_distill_refuses(top, index, kw, error, what):
+    with pytest.raises(error, match=what):
+        dmv.distill_top_logits(_logits(4, 7), top, index, **kw)
+
+
+# ------------------------------------------------------------------------------------------ the C entry points
+FAKE = 4096          # an address that is only looked at: every call below is refused before it would be read
+
+
+def _rows(**kw):
+    r = L.DmvCatRows(logits=FAKE, ld=8, rows=4, V=8, dtype=0, X=FAKE, x_period=4)
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+def _teacher(**kw):
+    t = L.DmvCatTeacher(logits=FAKE, index=FAKE, period=4, k=2, dtype=0, temperature=1.0)
+    for k, v in kw.items():
+        setattr(t, k, v)
+    return t
+
+
+BAD, UNSUPPORTED, WORKSPACE = L.E_BADARG, L.E_UNSUPPORTED, L.E_WORKSPACE
+ROWS_REFUSED = [(dict(rows=-1), BAD), (dict(V=0), BAD), (dict(ld=-1), BAD), (dict(logits=None), BAD), (dict(logits=FAKE + 2), BAD),
+                (dict(dtype=1, logits=FAKE + 1), BAD), (dict(x_period=0), BAD), (dict(M=FAKE, m_period=0), BAD),
+                (dict(sizes=FAKE, size_period=0), BAD), (dict(dtype=3), UNSUPPORTED), (dict(dtype=-1), UNSUPPORTED),
+                (dict(rows=1 << 31), UNSUPPORTED), (dict(V=0x7fffffff), UNSUPPORTED)]
+
+
+@pytest.mark.parametrize("kw, code", ROWS_REFUSED)
+def test_entry_points_refuse_rows(kw, code):
+    lib = L.lib()
+    r, t = C.byref(_rows(**kw)), C.byref(_teacher())
+    assert lib.dmv_cat_log_prob(r, FAKE, None, 0, None, None, None, None, 0, None) == code
+    assert lib.dmv_cat_log_prob_backward(r, FAKE, FAKE, None, 0, None, None, FAKE, 1 << 40, None) == code
+    assert lib.dmv_cat_distill(r, t, FAKE, FAKE, None, None, 0, FAKE, 1 << 40, None) == code
+    assert lib.dmv_cat_distill_backward(r, t, FAKE, 0, FAKE, FAKE, 1 << 40, None) == code
+    assert lib.dmv_cat_log_prob_ws_bytes(r, 1) == 0 and lib.dmv_cat_distill_ws_bytes(r) == 0
+
+
+@pytest.mark.parametrize("args, code", [
+    ((None, None, 0, None, None, None, None, 0), BAD),                   # nothing asked for
+    ((FAKE, None, -1, None, None, None, None, 0), BAD),
+    ((FAKE, None, 65, FAKE, FAKE, None, None, 0), UNSUPPORTED),
+    ((FAKE, None, 2, None, FAKE, None, None, 0), BAD),
+    ((FAKE, None, 2, FAKE, None, None, None, 0), BAD),
+    ((FAKE, None, 0, None, None, FAKE + 4, None, 0), BAD),               # misaligned stats
+    ((FAKE, None, 0, None, None, None, FAKE + 8, 0), BAD)])              # misaligned workspace
+def test_log_prob_entry_refuses(args, code):
+    assert L.lib().dmv_cat_log_prob(C.byref(_rows()), *args, None) == code
+
+
+def test_log_prob_entry_needs_x_and_workspace():
+    lib = L.lib()
+    assert lib.dmv_cat_log_prob(C.byref(_rows(X=None)), FAKE, None, 0, None, None, None, None, 0, None) == BAD
+    r = _rows(V=50000, ld=50000)
+    need = lib.dmv_cat_log_prob_ws_bytes(C.byref(r), 5)
+    assert need > 0 and need % 8 == 0
+    for ws, n in ((None, 0), (FAKE, need - 1)):
+        assert lib.dmv_cat_log_prob(C.byref(r), FAKE, None, 5, FAKE, FAKE, None, ws, n, None) == WORKSPACE
+
+
+@pytest.mark.parametrize("args, code", [
+    ((FAKE, FAKE, None, 0, None, None, FAKE, 7), BAD),                   # pitch below V
+    ((FAKE, FAKE, None, 0, None, FAKE, FAKE, 8), BAD),                   # gradient of alternatives that were not asked for
+    ((FAKE, FAKE, None, 65, FAKE, FAKE, FAKE, 8), UNSUPPORTED),
+    ((None, FAKE, None, 0, None, None, FAKE, 8), BAD),
+    ((FAKE, FAKE, None, 0, None, None, None, 8), BAD),
+    ((FAKE, FAKE, None, 0, None, None, FAKE + 1, 8), BAD)])
+def test_backward_entry_refuses(args, code):
+    assert L.lib().dmv_cat_log_prob_backward(C.byref(_rows()), *args, None) == code
+
+
+@pytest.mark.parametrize("kw, code", [
+    (dict(logits=None), BAD), (dict(index=None), BAD), (dict(period=0), BAD), (dict(k=0), BAD), (dict(k=257), UNSUPPORTED),
+    (dict(dtype=5), UNSUPPORTED), (dict(temperature=0.0), BAD), (dict(temperature=-1.0), BAD), (dict(temperature=float("nan")), BAD),
+    (dict(weight=FAKE, w_period=0), BAD), (dict(logits=FAKE + 1), BAD)])
+def test_distill_entry_refuses_teacher(kw, code):
+    lib = L.lib()
+    t = C.byref(_teacher(**kw))
+    assert lib.dmv_cat_distill(C.byref(_rows()), t, FAKE, FAKE, None, None, 0, FAKE, 1 << 30, None) == code
+    assert lib.dmv_cat_distill_backward(C.byref(_rows()), t, FAKE, 0, FAKE, FAKE, 8, None) == code
+
+
+def test_distill_entry_refuses_outputs_and_workspace():
+    lib = L.lib()
+    r, t = C.byref(_rows()), C.byref(_teacher())
+    need = lib.dmv_cat_distill_ws_bytes(r)
+    assert need >= 8
+    call = lambda loss=FAKE, stats=None, d=None, ld=8, ws=FAKE, n=need: lib.dmv_cat_distill(r, t, None, loss, stats, d, ld, ws, n, None)  # noqa: E731
+    assert call(loss=None) == BAD and call(d=FAKE, ld=7) == BAD and call(d=FAKE + 1) == BAD and call(stats=FAKE + 4) == BAD
+    assert call(ws=None) == WORKSPACE and call(n=need - 1) == WORKSPACE and call(ws=FAKE + 8) == WORKSPACE
+    big = C.byref(_rows(V=5000, ld=5000))
+    assert lib.dmv_cat_distill_backward(big, t, FAKE, 0, None, FAKE, 5000, None) == BAD      # long rows need their statistics
+    assert lib.dmv_cat_distill_backward(r, t, None, 0, FAKE, FAKE, 8, None) == BAD
