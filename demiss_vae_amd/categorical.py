@@ -13,7 +13,6 @@ another model gave:
 
 Both are differentiable with respect to the logits (float32, bfloat16 or float16), run on the current stream, allocate
 through torch only and record into HIP graphs.  There is no CPU path."""
-import contextlib
 import ctypes as C
 from typing import NamedTuple, Optional
 
@@ -110,23 +109,41 @@ def _row_args(logits, X, M, sizes):
     return r, keep
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device):
-    """Launches go to the current stream of the tensors' device."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _set_logits(r, logits):
+def _set_logits(r, logits, keep):
+    """The logits of a call: its rows in `r`; what they had to be copied to is kept alive with the call's other arrays."""
     flat, r.rows, _, r.ld = _rows(logits)
     r.logits = flat.data_ptr()
-    return flat
+    if flat is not logits:
+        keep.append(flat)
 
 
-def _forward(logits, r, want_lp, entropy, top, want_stats):
-    lib, dev, lead = L.lib(), logits.device, logits.shape[:-1]
-    flat = _set_logits(r, logits)
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on_device(f):
+    """Runs f(device, ...) with the tensors' device as the current one: launches go to its current stream."""
+    def call(device, *args):
+        if device.index == torch._C._cuda_getDevice():
+            return f(device, *args)
+        with torch.cuda.device(device):
+            return f(device, *args)
+    return call
+
+
+def _backward(f):
+    """A backward pass in terms of kernel launches: fine as it is, unless autograd records it (create_graph=True)."""
+    once = torch.autograd.function.once_differentiable(f)
+
+    def backward(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
+    return staticmethod(backward)
+
+
+@_on_device
+def _log_prob(dev, logits, r, keep, want_lp, entropy, top, want_stats):
+    lib, lead = L.lib(), logits.shape[:-1]
+    _set_logits(r, logits, keep)
     f32 = torch.float32
     lp = torch.empty(lead, dtype=f32, device=dev) if want_lp else None
     ent = torch.empty(lead, dtype=f32, device=dev) if entropy else None
@@ -135,38 +152,37 @@ def _forward(logits, r, want_lp, entropy, top, want_stats):
     stats = torch.empty((r.rows, 4), dtype=f32, device=dev) if want_stats else None
     n_ws = lib.dmv_cat_log_prob_ws_bytes(C.byref(r), top) if r.V > L.CAT_SHORT_ROW else 0
     ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
-    L.check(lib.dmv_cat_log_prob(C.byref(r), L.addr(lp), L.addr(ent), top, L.addr(top_lp), L.addr(top_idx), L.addr(stats), L.addr(ws), n_ws,
-                                 L.stream_ptr()))
-    del flat
+    L.check(lib.dmv_cat_log_prob(C.byref(r), L.addr(lp), L.addr(ent), top, L.addr(top_lp), L.addr(top_idx), L.addr(stats),
+                                 L.addr(ws), n_ws, _stream(dev)))
     return lp, ent, top_lp, top_idx, stats
+
+
+@_on_device
+def _log_prob_backward(dev, logits, r, stats, g_lp, g_ent, top, top_idx, g_top):
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    L.check(L.lib().dmv_cat_log_prob_backward(C.byref(r), L.addr(stats), L.addr(g_lp), L.addr(g_ent), top, L.addr(top_idx),
+                                              L.addr(g_top), L.addr(d), r.V, _stream(dev)))
+    return d
 
 
 class _LogProb(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, r, keep, want_lp, entropy, top):
-        with _on(logits.device):
-            lp, ent, top_lp, top_idx, stats = _forward(logits, r, want_lp, entropy, top, True)
+        lp, ent, top_lp, top_idx, stats = _log_prob(logits.device, logits, r, keep, want_lp, entropy, top, True)
         ctx.r, ctx.keep, ctx.top = r, keep, top
         ctx.save_for_backward(logits, stats, top_idx)
         ctx.set_materialize_grads(False)
-        if top_idx is not None:
+        if top:
             ctx.mark_non_differentiable(top_idx)
         return lp, ent, top_lp, top_idx
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, g_lp, g_ent, g_top, _):
-        if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None, None, None, None
-        logits, stats, top_idx = ctx.saved_tensors
-        r = ctx.r
-        g_lp, g_ent, g_top = (None if g is None else g.float().contiguous() for g in (g_lp, g_ent, g_top))
-        with _on(logits.device):
-            flat = _set_logits(r, logits)
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            L.check(L.lib().dmv_cat_log_prob_backward(C.byref(r), L.addr(stats), L.addr(g_lp), L.addr(g_ent), ctx.top, L.addr(top_idx),
-                                                      L.addr(g_top), L.addr(d), r.V, L.stream_ptr()))
-            del flat
+        d = None
+        if g_lp is not None or g_ent is not None or g_top is not None:
+            logits, stats, top_idx = ctx.saved_tensors
+            g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
+            d = _log_prob_backward(logits.device, logits, ctx.r, stats, g_lp, g_ent, ctx.top, top_idx, g_top)
         return d, None, None, None, None, None
 
 
@@ -189,52 +205,52 @@ def categorical_log_prob(logits, X=None, M=None, *, sizes=None, entropy=False, t
     _need_gpu(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return CategoricalLogProb(*_LogProb.apply(logits, r, keep, X is not None, bool(entropy), top))
-    with _on(logits.device):
-        return CategoricalLogProb(*_forward(logits, r, X is not None, bool(entropy), top, False)[:4])
+    return CategoricalLogProb(*_log_prob(logits.device, logits, r, keep, X is not None, bool(entropy), top, False)[:4])
+
+
+@_on_device
+def _distill(dev, logits, r, t, keep, training):
+    lib = L.lib()
+    _set_logits(r, logits, keep)
+    per_row = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if training else None
+    stats = torch.empty((r.rows, 4), dtype=torch.float32, device=dev) if training and r.V > L.CAT_SHORT_ROW else None
+    n_ws = lib.dmv_cat_distill_ws_bytes(C.byref(r))
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+    L.check(lib.dmv_cat_distill(C.byref(r), C.byref(t), L.addr(per_row), L.addr(loss), L.addr(stats), L.addr(d), r.V, L.addr(ws), n_ws,
+                                _stream(dev)))
+    return loss, per_row, stats, d
+
+
+@_on_device
+def _distill_backward(dev, logits, r, t, g, stats, d):
+    unless_one = d is not None
+    if d is None:
+        d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    L.check(L.lib().dmv_cat_distill_backward(C.byref(r), C.byref(t), L.addr(g), unless_one, L.addr(stats), L.addr(d), r.V, _stream(dev)))
+    return d
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, r, t, keep):
-        lib, dev = L.lib(), logits.device
-        training = ctx.needs_input_grad[0]
-        with _on(dev):
-            flat = _set_logits(r, logits)
-            per_row = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if training else None
-            stats = torch.empty((r.rows, 4), dtype=torch.float32, device=dev) if training and r.V > L.CAT_SHORT_ROW else None
-            n_ws = lib.dmv_cat_distill_ws_bytes(C.byref(r))
-            ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-            L.check(lib.dmv_cat_distill(C.byref(r), C.byref(t), L.addr(per_row), L.addr(loss), L.addr(stats), L.addr(d), r.V, L.addr(ws), n_ws,
-                                        L.stream_ptr()))
-            del flat
-        ctx.r, ctx.t, ctx.keep, ctx.d = r, t, keep, d
+        loss, per_row, stats, ctx.d = _distill(logits.device, logits, r, t, keep, True)
+        ctx.r, ctx.t, ctx.keep = r, t, keep
         ctx.save_for_backward(logits, stats)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(per_row)
         return loss, per_row
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_backward
     def backward(ctx, g, _):
         if g is None:
             return None, None, None, None
         logits, stats = ctx.saved_tensors
-        r = ctx.r
-        g = g.float().contiguous()
         # the forward pass has written the gradient for g = 1 (a loss that is not scaled further): any other g forms it
         # again from the logits, on the device; a second backward pass has a gradient of its own
         d, ctx.d = ctx.d, None
-        first = d is not None
-        with _on(logits.device):
-            if not first:
-                d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            flat = _set_logits(r, logits)
-            L.check(L.lib().dmv_cat_distill_backward(C.byref(r), C.byref(ctx.t), L.addr(g), 1 if first else 0, L.addr(stats), L.addr(d), r.V,
-                                                     L.stream_ptr()))
-            del flat
-        return d, None, None, None
+        return _distill_backward(logits.device, logits, ctx.r, ctx.t, g, stats, d), None, None, None
 
 
 def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None, temperature=1.0):
@@ -276,4 +292,6 @@ def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None
         t.weight = weight.data_ptr()
         keep.append(weight)
     _need_gpu(logits)
-    return _Distill.apply(logits, r, t, keep)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Distill.apply(logits, r, t, keep)
+    return _distill(logits.device, logits, r, t, keep, False)[:2]

@@ -20,6 +20,7 @@ constexpr float kClampD = -256.f;        // 2^d is 0 below: keeps 0 * (-inf) out
 constexpr float kNearCertain = 0.0625f;  // below this r the largest category's thread sums its other terms again
 constexpr int kMaxTop = DMV_CAT_MAX_TOP;
 constexpr int kMaxTeacher = DMV_CAT_MAX_TEACHER;
+constexpr int kMaxParts = 64;            // workgroups per row: a lane of the join each
 
 // ------------------------------------------------------------------------------------------ elements
 // 16 bytes of a row whose address is only element-aligned: one 16-byte access (the hardware takes any alignment)
@@ -638,9 +639,10 @@ __device__ __forceinline__ void block_sum3(float& p, float& q, float& w, BlockRe
 // running (max, sum, entropy sum) of one thread
 struct Online {
   float m = -INFINITY, s = 0.f, t = 0.f;
+  // N values, the largest of them mx
   template <int N, bool ENT>
-  __device__ __forceinline__ void add(const float* v, float c) {
-    const float mn = max_of<N>(v, m);
+  __device__ __forceinline__ void add(const float* v, float mx, float c) {
+    const float mn = max3(mx, m, m);
     const float ref = mn == -INFINITY ? 0.f : mn;
     const float shift = fmaxf((m - ref) * c, kClampD), f = exp2_hw(shift);
     if (ENT) t = f * fmaf(s, shift, t);
@@ -688,140 +690,192 @@ __device__ __forceinline__ void block_join(const Online& on, float c, BlockRed<N
 
 constexpr int kRowThreads = 256;
 constexpr int kUnroll = 4;              // slots in flight per thread
-constexpr int kGroups = 16;             // slot groups whose maxima a thread keeps for the selection
-constexpr int kCand = 1024;             // candidates of a selection
+constexpr int kGroups = 8;              // slot groups whose maxima a thread keeps for the selection
+constexpr int kCand = 512;              // candidates of a selection
 
-template <int DT, bool TOP>
-struct RowShared {
-  BlockRed<kRowThreads> red;
-  int holder;
-};
-template <int DT>
+// Candidates of a selection: key in the upper half, ~index in the lower, so that the larger number is the better one.
+typedef unsigned long long cand_t;
+__device__ __forceinline__ cand_t candidate(uint32_t key, uint32_t index) { return ((cand_t)key << 32) | (uint32_t)~index; }
+constexpr int kCandPad = 64;
+
 struct TopShared {
-  float gm[kGroups][kRowThreads];
+  float gm[kGroups][kRowThreads];      // largest value of a thread's slot group
   float tmax[kRowThreads];
-  uint2 cand[kCand];
-  int count;
+  uint16_t list[kGroups * kRowThreads];
+  cand_t cand[kCand + kCandPad];
+  int groups, count;
   unsigned long long best[kRowThreads / 64];
   int scan[kRowThreads / 64];
 };
 
+// largest t with count(key >= t) >= k over the wavefront's G keys a lane (0 if there are fewer), or a smaller one that not
+// many more than k keys reach: bit by bit, down to the bits that differ between values of the type.  `top` is the largest
+// key: most often k keys share its exponent, and the search starts below that.
+template <int DT, int G>
+__device__ __forceinline__ uint32_t lower_bound_of(const uint32_t* g, uint32_t top, int k) {
+  auto count = [&](uint32_t t) {
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < G; ++w) c += __popcll(__ballot(g[w] >= t));
+    return c;
+  };
+  const uint32_t start = top & 0xff800000u;
+  int c = count(start);
+  uint32_t tau = c >= k ? start : 0u;
+  const int enough = k + (k >> 2) + 1;
+  for (int bit = c >= k ? 22 : 31; bit >= Elem<DT>::kOpenBits && !(tau != 0u && c <= enough); --bit) {
+    const uint32_t t = tau | (1u << bit);
+    const int ct = count(t);
+    if (ct >= k) {
+      tau = t;
+      c = ct;
+    }
+  }
+  return tau;
+}
+
+// Ranks the `have` candidates of a list with room for kCandPad more by counting the better ones, and emits those of rank
+// below k.  Few candidates are counted by up to 16 lanes each: have^2 / NT comparisons a thread.
+template <int NT, typename Emit>
+__device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, Emit emit) {
+  const int tid = threadIdx.x;
+  if (tid < kCandPad) cand[have + tid] = 0;
+  __syncthreads();
+  int sh = 0;
+  while (sh < 4 && (have << (sh + 1)) <= NT) ++sh;
+  const int lanes = 1 << sh, sub = tid & (lanes - 1);
+  for (int i0 = 0; i0 < have; i0 += NT >> sh) {
+    const int i = i0 + (tid >> sh);
+    const cand_t me = i < have ? cand[i] : 0;
+    int rank = 0;
+    for (int j = sub; j < have; j += 4 * lanes) {
+      cand_t o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = cand[j + q * lanes];      // past the end: 0, better than nothing
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rank += o[q] > me ? 1 : 0;
+    }
+    if (sh >= 1) rank += (int)dpp_move_u<0xB1>((uint32_t)rank);
+    if (sh >= 2) rank += (int)dpp_move_u<0x4E>((uint32_t)rank);
+    if (sh >= 3) rank += (int)dpp_move_u<0x141>((uint32_t)rank);
+    if (sh >= 4) rank += (int)dpp_move_u<0x140>((uint32_t)rank);
+    if (i < have && sub == 0 && rank < k) emit(rank, (uint32_t)(me >> 32), (int)~(uint32_t)me);
+  }
+}
+
 // The selection's result goes through `emit(rank, key, index)`.
 //
-// Every thread knows the largest value of each of its slot groups.  tau, the k-th largest of the threads' largest values
-// (256 of them), is a lower bound of the k-th largest element, and only the groups whose largest value reaches it are read
-// again: about k (1 + k / 512) elements of an ordinary row.  They are ranked by counting.  Rows with more candidates
-// than fit (many equal values) take the ordered scan below, and in the worst case one pass over the row per rank.
+// Every thread knows the largest value of each of its slot groups.  tau, at most the k-th largest of the threads' largest
+// values (256 of them), is a lower bound of the k-th largest element, so only groups whose largest value reaches tau hold
+// any of the k: these are listed, read again with a slot per thread, and the elements that reach tau - little more than k
+// in an ordinary row - are ranked by counting.  Rows with more candidates than fit (many equal values) take the
+// ordered scan below, and in the worst case one pass over the listed groups per rank.
 template <int DT, int VEC, typename Emit>
-__device__ void block_top(TopShared<DT>& sh, const char* p, int V, int n, int s0, int s1, int gsz, int k, float tmax, Emit emit) {
+__device__ void block_top(TopShared& sh, const char* p, int V, int n, int s0, int s1, int gsz, int k, float m, float tmax, Emit emit) {
   constexpr int NT = kRowThreads;
   const int tid = threadIdx.x, lane = tid & 63;
-  if (tid == 0) sh.count = 0;
+  const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
+  if (tid == 0) sh.count = sh.groups = 0;
   sh.tmax[tid] = tmax;
   __syncthreads();
   uint32_t g[NT / 64];
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) g[w] = order_key(sh.tmax[64 * w + lane]);
-  // largest t with count(key >= t) >= k, bit by bit, down to the bits that differ between values of the type
-  uint32_t tau = 0;
-  for (int bit = 31; bit >= Elem<DT>::kOpenBits; --bit) {
-    const uint32_t t = tau | (1u << bit);
-    int cnt = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) cnt += __popcll(__ballot(g[w] >= t));
-    if (cnt >= k) tau = t;
-    if (cnt == k) break;
-  }
+  uint32_t tau = lower_bound_of<DT, NT / 64>(g, order_key(m), k);
   if (tau <= kKeyMinusInf) tau = kKeyMinusInf + 1;   // -inf is no alternative
-  auto each = [&](uint32_t lowest, auto f) {          // f(key, index) of this thread's elements with key >= lowest
-    if (order_key(tmax) < lowest) return;
-    const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
-    for (int q = 0; q < groups; ++q) {
-      if (order_key(sh.gm[q][tid]) < lowest) continue;
-      for (int i = 0; i < gsz; ++i) {
-        const int s = s0 + tid + NT * (q * gsz + i);
-        if (s >= s1) break;
-        float v[VEC];
-        const int b = slot_base<VEC>(s, V);
-        slot_load<DT, VEC>(p, b, v);
+  // the groups with a value that reaches `lowest`, in sh.list
+  auto list_groups = [&](uint32_t lowest) {
+    if (order_key(tmax) >= lowest)
+      for (int q = 0; q < groups; ++q)
+        if (order_key(sh.gm[q][tid]) >= lowest) sh.list[atomicAdd(&sh.groups, 1)] = (uint16_t)(q * NT + tid);
+    __syncthreads();
+  };
+  // f(keys that reach `lowest`, index of the slot's first element, bits of those elements) for the listed groups
+  auto each_slot = [&](uint32_t lowest, auto f) {
+    const int total = sh.groups * gsz;
+    for (int j = tid; j < total; j += NT) {
+      const int l = j / gsz, at = sh.list[l];
+      const int s = s0 + (at & (NT - 1)) + NT * (at / NT * gsz + (j - l * gsz));
+      if (s >= s1) continue;
+      float v[VEC];
+      const int b = slot_base<VEC>(s, V);
+      slot_load<DT, VEC>(p, b, v);
+      uint32_t key[VEC], bits = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const uint32_t key = order_key(v[e]);
-          if (b + e >= s * VEC && b + e < n && key >= lowest) f(key, b + e);
-        }
+      for (int e = 0; e < VEC; ++e) {
+        key[e] = order_key(v[e]);
+        if (b + e >= s * VEC && b + e < n && key[e] >= lowest) bits |= 1u << e;
       }
+      if (bits) f(key, b, bits);
     }
   };
   auto collect = [&](uint32_t lowest) {
-    each(lowest, [&](uint32_t key, int i) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < kCand) sh.cand[at] = make_uint2(key, (uint32_t)i);
+    list_groups(lowest);
+    each_slot(lowest, [&](const uint32_t* key, int b, uint32_t bits) {
+      int at = atomicAdd(&sh.count, __popc(bits));
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if ((bits >> e) & 1u) {
+          if (at < kCand) sh.cand[at] = candidate(key[e], (uint32_t)(b + e));
+          ++at;
+        }
     });
     __syncthreads();
     return sh.count;
   };
-  auto rank_all = [&](int have) {                     // ranks of all candidates, those below k are emitted
-    for (int i = tid; i < have; i += NT) {
-      const uint2 me = sh.cand[i];
-      int rank = 0;
-      for (int j = 0; j < have; ++j) {
-        const uint2 o = sh.cand[j];
-        rank += (o.x > me.x || (o.x == me.x && o.y < me.y)) ? 1 : 0;
-      }
-      if (rank < k) emit(rank, me.x, (int)me.y);
-    }
-  };
   int have = collect(tau);
   int done;
   if (have <= kCand) {
-    rank_all(have);
+    rank_candidates<NT>(sh.cand, have, k, emit);
     done = have;
   } else {
-    // many values reach tau: make it the key of the k-th largest of the threads' values itself, so that those equal to
-    // it can be told from those above
-    uint32_t kth = 0xffffffffu;
+    // many values reach tau: make it the key of the k-th largest of the threads' values itself (where k threads have
+    // one), so that those equal to it can be told from those above
+    auto reach = [&](uint32_t t) {
+      int c = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) kth = (g[w] >= tau && g[w] < kth) ? g[w] : kth;
-    kth = ~gmax_u<64>(~kth);
-    if (kth != 0xffffffffu) tau = kth;
+      for (int w = 0; w < NT / 64; ++w) c += __popcll(__ballot(g[w] >= t));
+      return c;
+    };
+    for (uint32_t t = tau; reach(t) >= k;) {       // the next of the threads' values, as long as k reach it
+      uint32_t next = 0xffffffffu;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) next = (g[w] >= t && g[w] < next) ? g[w] : next;
+      next = ~gmax_u<64>(~next);
+      if (reach(next) < k) break;
+      tau = next;
+      t = next + 1u;
+    }
     const uint32_t above = tau + 1u;
     __syncthreads();
-    if (tid == 0) sh.count = 0;
+    if (tid == 0) sh.count = sh.groups = 0;
     __syncthreads();
     have = collect(above);
     if (have <= kCand) {
-      rank_all(have);
+      rank_candidates<NT>(sh.cand, have, k, emit);
       done = have < k ? have : k;
       // elements equal to tau, lowest index first: a round covers NT consecutive slots, in index order by thread
       for (int it = 0; done < k && s0 + NT * it < s1; ++it) {
         const int s = s0 + tid + NT * it;
-        uint32_t bits = 0, key0 = 0;
+        uint32_t bits = 0;
         const int b = slot_base<VEC>(s < s1 ? s : s1 - 1, V);
         if (s < s1) {
           float v[VEC];
           slot_load<DT, VEC>(p, b, v);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const uint32_t key = order_key(v[e]);
-            if (b + e >= s * VEC && b + e < n && key >= tau && key < above) {
-              bits |= 1u << e;
-              key0 = key;
-            }
-          }
+          for (int e = 0; e < VEC; ++e)
+            if (b + e >= s * VEC && b + e < n && order_key(v[e]) == tau) bits |= 1u << e;
         }
-        const int c = __popc(bits);
-        int before = 0;      // inclusive scan over the wavefront
-        int run = c;
+        int run = __popc(bits);     // inclusive scan over the wavefront
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
           const int up = __shfl_up(run, off);
           if (lane >= off) run += up;
         }
-        before = run - c;
         __syncthreads();
         if (lane == 63) sh.scan[tid >> 6] = run;
         __syncthreads();
-        int total = 0;
+        int before = run - __popc(bits), total = 0;
 #pragma unroll
         for (int w = 0; w < NT / 64; ++w) {
           if (w < (tid >> 6)) before += sh.scan[w];
@@ -830,7 +884,7 @@ __device__ void block_top(TopShared<DT>& sh, const char* p, int V, int n, int s0
         int rank = done + before;
         for (int e = 0; e < VEC; ++e)
           if ((bits >> e) & 1u) {
-            if (rank < k) emit(rank, key0, b + e);
+            if (rank < k) emit(rank, tau, b + e);
             ++rank;
           }
         done += total;
@@ -840,9 +894,12 @@ __device__ void block_top(TopShared<DT>& sh, const char* p, int V, int n, int s0
       unsigned long long last = ~0ull;
       for (done = 0; done < k; ++done) {
         unsigned long long best = 0;
-        each(tau, [&](uint32_t key, int i) {
-          const unsigned long long o = ((unsigned long long)key << 32) | (uint32_t)~i;
-          if (o < last && o > best) best = o;
+        each_slot(above, [&](const uint32_t* key, int b, uint32_t bits) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const unsigned long long o = ((unsigned long long)key[e] << 32) | (uint32_t)~(b + e);
+            if (((bits >> e) & 1u) && o < last && o > best) best = o;
+          }
         });
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
@@ -868,7 +925,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
   constexpr int NT = kRowThreads, VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
   __shared__ BlockRed<NT> red;
   __shared__ int holder;
-  __shared__ typename std::conditional<TOP, TopShared<DT>, int>::type top_sh;
+  __shared__ typename std::conditional<TOP, TopShared, int>::type top_sh;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x - (int)(row * a.parts);
@@ -879,8 +936,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
   }
   const int n = row_size(a.r, row), V = a.r.V;
   const int ns = (n + VEC - 1) / VEC;
-  // parts are whole rounds of NT slots, so that their accesses stay contiguous
-  const int rounds = (ns + NT - 1) / NT, per = ((rounds + a.parts - 1) / a.parts) * NT;
+  const int per = ((ns + a.parts - 1) / a.parts + 63) & ~63;      // whole wavefronts of slots
   const int s0 = part * per < ns ? part * per : ns, s1 = s0 + per < ns ? s0 + per : ns;
   const char* p = a.r.x + row * a.r.ld * ES;
   int gsz = (s1 - s0 + NT * kGroups - 1) / (NT * kGroups);    // slots per group of the selection
@@ -906,8 +962,9 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
           if (sq >= s1 || b + e < sq * VEC || b + e >= n) v[q * VEC + e] = -INFINITY;
       }
     }
+    const float mx = max_of<kUnroll * VEC>(v, -INFINITY);
     if constexpr (TOP) {
-      gmx = max_of<kUnroll * VEC>(v, gmx);
+      gmx = max3(mx, gmx, gmx);
       in_group += kUnroll;
       if (in_group == gsz) {
         top_sh.gm[group++][tid] = gmx;
@@ -915,7 +972,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
         in_group = 0;
       }
     }
-    on.template add<kUnroll * VEC, ENT>(v, a.c);
+    on.template add<kUnroll * VEC, ENT>(v, mx, a.c);
   }
   if constexpr (TOP) {
     const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
@@ -942,7 +999,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
     if (tid == 0) a.part[row * a.parts + part] = f32x4{m, r, u, 0.f};
     if constexpr (TOP) {
       uint2* o = a.part_top + (row * a.parts + part) * a.top;
-      block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, on.m,
+      block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m,
                          [&](int rank, uint32_t key, int i) { o[rank] = make_uint2(key, (uint32_t)i); });
     }
     return;
@@ -969,7 +1026,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
       }
       return;
     }
-    block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, on.m, [&](int rank, uint32_t key, int i) {
+    block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m, [&](int rank, uint32_t key, int i) {
       a.top_idx[row * a.top + rank] = i;
       a.top_lp[row * a.top + rank] = i < 0 ? -INFINITY : (key_value(key) - m) - logs;
     });
@@ -990,9 +1047,14 @@ __device__ __forceinline__ void join_parts(const f32x4* part, int parts, float c
   u = gsum<64>(b);
 }
 
+// The parts' ordered lists hold parts * k candidates.  If j = ceil(k / parts) of every part reach tau, k elements do: tau
+// = the smallest of the parts' j-th keys.  Those that reach it are ranked by counting.
+constexpr int kJoinThreads = 256;
 template <int DT>
-__global__ void __launch_bounds__(64) k_cat_fwd_join(Fwd a) {
-  const int lane = threadIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) k_cat_fwd_join(Fwd a) {
+  __shared__ cand_t cand[kMaxParts * kMaxTop + kCandPad];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const bool seen = row_seen(a.r, row);
   if (!seen && !a.entropy && !a.top) return;        // the parts' launch has written it
@@ -1003,7 +1065,8 @@ __global__ void __launch_bounds__(64) k_cat_fwd_join(Fwd a) {
   const bool empty = m == -INFINITY && !(r != r);
   const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
   const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
-  if (lane == 0) {
+  if (tid == 0) {
+    count = 0;
     if (a.log_prob) {
       float lp = 0.f;
       if (seen) {
@@ -1016,23 +1079,32 @@ __global__ void __launch_bounds__(64) k_cat_fwd_join(Fwd a) {
     if (a.stats) a.stats[row] = f32x4{m, inv_s, logs, H};
   }
   if (!a.top) return;
-  const bool bad = logs != logs;
-  // merge of the parts' ordered lists: lane = part, its head against the others'
-  const uint2* list = a.part_top + (row * a.parts + lane) * (int64_t)a.top;
-  int head = 0;
-  uint2 cur = lane < a.parts ? list[0] : make_uint2(0u, 0u);
-  for (int t = 0; t < a.top; ++t) {
-    const uint32_t top = gmax_u<64>(cur.x);
-    const uint32_t low = ~gmax_u<64>((cur.x == top) ? ~cur.y : 0u);
-    if (top != 0u && cur.x == top && cur.y == low) {
-      ++head;
-      cur = head < a.top ? list[head] : make_uint2(0u, 0u);
+  if (logs != logs) {
+    for (int j = tid; j < a.top; j += kJoinThreads) {
+      a.top_idx[row * a.top + j] = -1;
+      a.top_lp[row * a.top + j] = NAN;
     }
-    if (lane == 0) {
-      const bool none = top == 0u || bad;
-      a.top_idx[row * a.top + t] = none ? -1 : (int64_t)low;
-      a.top_lp[row * a.top + t] = bad ? NAN : (none ? -INFINITY : (key_value(top) - m) - logs);
-    }
+    return;
+  }
+  const uint2* list = a.part_top + row * a.parts * a.top;
+  const int jth = (a.top + a.parts - 1) / a.parts - 1;
+  uint32_t tau = lane < a.parts ? list[lane * a.top + jth].x : 0xffffffffu;
+  tau = ~gmax_u<64>(~tau);
+  if (tau == 0u) tau = 1u;              // key 0: past the end of a part's list
+  __syncthreads();
+  for (int j = tid; j < a.parts * a.top; j += kJoinThreads) {
+    const uint2 o = list[j];
+    if (o.x >= tau) cand[atomicAdd(&count, 1)] = candidate(o.x, o.y);
+  }
+  __syncthreads();
+  const int have = count;
+  rank_candidates<kJoinThreads>(cand, have, a.top, [&](int rank, uint32_t key, int i) {
+    a.top_idx[row * a.top + rank] = i;
+    a.top_lp[row * a.top + rank] = (key_value(key) - m) - logs;
+  });
+  for (int j = have + tid; j < a.top; j += kJoinThreads) {
+    a.top_idx[row * a.top + j] = -1;
+    a.top_lp[row * a.top + j] = -INFINITY;
   }
 }
 
@@ -1397,7 +1469,6 @@ __global__ void __launch_bounds__(kLossThreads) k_cat_loss(const double* part, i
 // ------------------------------------------------------------------------------------------ host side
 constexpr int64_t kMaxGrid = 0x7fffffffll;
 constexpr int kSmallMax = DMV_CAT_SHORT_ROW;   // longest row of the register kernels of short rows
-constexpr int kMaxParts = 64;           // a join's lane per part
 
 int check_rows(const DmvCatRows* r) {
   if (!r || r->rows < 0 || r->V < 1 || r->ld < 0) return DMV_E_BADARG;
@@ -1519,7 +1590,7 @@ extern "C" int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* ent
   by_type(r->dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     launch_fwd_rows<DT>(a, entropy != nullptr, st);
-    if (a.parts > 1) k_cat_fwd_join<DT><<<(unsigned)r->rows, 64, 0, st>>>(a);
+    if (a.parts > 1) k_cat_fwd_join<DT><<<(unsigned)r->rows, kJoinThreads, 0, st>>>(a);
   });
   DMV_HIP_CHECK_LAUNCH();
   return DMV_OK;

@@ -387,6 +387,19 @@ def test_selection_when_few_threads_hold_all_large_values(rows, dtype, slot):
         check_log_prob(x, top=7, entropy=True)
 
 
+@pytest.mark.parametrize("dtype, slot", [(torch.float32, 4), (torch.bfloat16, 8), (torch.float16, 8)], ids=str)
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("threads", [1, 3, 20])
+def test_selection_when_few_threads_have_any_value(rows, threads, dtype, slot):
+    """fewer threads with a finite value than alternatives asked for, and more such values than the candidate list holds"""
+    V = 65536
+    s = torch.arange(V, device="cuda") // slot % 256
+    for v in (make((rows, V), torch.float32, seed=3), torch.full((rows, V), -1.0, device="cuda"), make((rows, V), torch.float32).round()):
+        x = torch.where(s < threads, v, -math.inf).to(dtype)
+        check_log_prob(x, top=64)
+        check_log_prob(x, top=5, entropy=True)
+
+
 # ------------------------------------------------------------------------------------------ differences
 @pytest.mark.parametrize("V", [3, 50, 1500, 40000])
 def test_gradient_against_differences(V):
