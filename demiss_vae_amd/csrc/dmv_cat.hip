@@ -665,30 +665,53 @@ struct Online {
   }
 };
 
+// (m, r, u) of the union of R sets with those of their own, one a lane (r = -1: an empty set)
+template <int R>
+__device__ __forceinline__ void join_sets(float& m, float& r, float& u, float c) {
+  const float top = gmax<R>(m), ref = top == -INFINITY ? 0.f : top;
+  const float shift = fmaxf((m - ref) * c, kClampD), f = exp2_hw(shift);
+  const bool holds = m == top && m != -INFINITY;
+  const float others = gsum<R>(holds ? r : f * (1.f + r));
+  u = gsum<R>(f * (u - (1.f + r) * shift));
+  r = others + (gsum<R>(holds ? 1.f : 0.f) - 1.f);
+  m = top;
+}
+
 // Joins the threads' partial results; on return (m, r, u) are the same in every thread.
 //   resum(holder): sum over x < m of 2^(c (x - m)) over this thread's share of the elements that thread `holder` had
+template <int NT>
+struct JoinShared {
+  f32x4 wave[NT / 64];
+  float again[NT / 64];
+};
 template <int NT, bool ENT, typename ReSum>
-__device__ __forceinline__ void block_join(const Online& on, float c, BlockRed<NT>& red, int* holder, float& m, float& r, float& u,
-                                           ReSum resum) {
-  m = block_max<NT>(on.m, red);
-  const float ref = m == -INFINITY ? 0.f : m;
-  const float shift = fmaxf((on.m - ref) * c, kClampD), f = exp2_hw(shift);
-  const bool holds = on.m == m;
-  const float mine = holds ? on.s - 1.f : on.s * f;
-  float a = mine, b = ENT ? -f * fmaf(on.s, shift, on.t) : 0.f, h = holds ? 1.f : 0.f;
-  if (holds) *holder = threadIdx.x;
-  block_sum3<NT>(a, b, h, red);
-  r = a + (h - 1.f);
-  u = b;
-  if (m == -INFINITY && !(r != r)) r = -1.f;      // nothing of non-zero probability
-  else if (r < kNearCertain) {                    // one thread holds the largest: its sum has rounded the rest away
-    float again = resum(*holder, ref) + (holds ? 0.f : mine), z0 = 0.f, z1 = 0.f;
-    block_sum3<NT>(again, z0, z1, red);
-    r = again;
+__device__ __forceinline__ void block_join(const Online& on, float c, JoinShared<NT>& sh, float& m, float& r, float& u, ReSum resum) {
+  constexpr int W = NT / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float wm = gmax<64>(on.m), wref = wm == -INFINITY ? 0.f : wm;
+  const float shift = fmaxf((on.m - wref) * c, kClampD), f = exp2_hw(shift);
+  const bool holds = on.m == wm;
+  const unsigned long long who = __ballot(holds);
+  const float a = gsum<64>(holds ? on.s - 1.f : on.s * f), b = ENT ? -gsum<64>(f * fmaf(on.s, shift, on.t)) : 0.f;
+  if (lane == 0) sh.wave[wave] = f32x4{wm, wm == -INFINITY && a == a ? -1.f : a + ((float)__popcll(who) - 1.f), b,
+                                       __int_as_float(wave * 64 + __ffsll(who) - 1)};
+  __syncthreads();
+  const f32x4 mine = sh.wave[lane & (W - 1)];
+  m = mine[0], r = mine[1], u = mine[2];
+  join_sets<W>(m, r, u, c);
+  if (m == -INFINITY && r == r) r = -1.f;          // nothing of non-zero probability
+  else if (r < kNearCertain) {                     // one thread holds the largest: its sum has rounded the rest away
+    const int w = __ffsll(__ballot(mine[0] == m)) - 1, holder = __float_as_int(__shfl(mine[3], w));
+    const float mshift = fmaxf((on.m - m) * c, kClampD);
+    const float again = gsum<64>(resum(holder, m) + ((int)threadIdx.x == holder ? 0.f : on.s * exp2_hw(mshift)));
+    if (lane == 0) sh.again[wave] = again;
+    __syncthreads();
+    r = gsum<W>(sh.again[lane & (W - 1)]);
   }
 }
 
 constexpr int kRowThreads = 256;
+constexpr int kWideThreads = 1024;      // few rows
 constexpr int kUnroll = 4;              // slots in flight per thread
 constexpr int kGroups = 8;              // slot groups whose maxima a thread keeps for the selection
 constexpr int kCand = 512;              // candidates of a selection
@@ -696,16 +719,19 @@ constexpr int kCand = 512;              // candidates of a selection
 // Candidates of a selection: key in the upper half, ~index in the lower, so that the larger number is the better one.
 typedef unsigned long long cand_t;
 __device__ __forceinline__ cand_t candidate(uint32_t key, uint32_t index) { return ((cand_t)key << 32) | (uint32_t)~index; }
-constexpr int kCandPad = 64;
+constexpr int kCandPad = 128;
 
+constexpr int kMaxima = 4;              // largest values a lane holds in the search for the bound: 256 in all
+template <int NT>
 struct TopShared {
-  float gm[kGroups][kRowThreads];      // largest value of a thread's slot group
-  float tmax[kRowThreads];
-  uint16_t list[kGroups * kRowThreads];
+  float gm[kGroups][NT];               // largest value of a thread's slot group
+  float tmax[NT];
+  uint16_t list[kGroups * NT];
   cand_t cand[kCand + kCandPad];
   int groups, count;
-  unsigned long long best[kRowThreads / 64];
-  int scan[kRowThreads / 64];
+  uint32_t tau;
+  cand_t best[NT / 64];
+  int scan[NT / 64];
 };
 
 // largest t with count(key >= t) >= k over the wavefront's G keys a lane (0 if there are fewer), or a smaller one that not
@@ -739,6 +765,7 @@ __device__ __forceinline__ uint32_t lower_bound_of(const uint32_t* g, uint32_t t
 template <int NT, typename Emit>
 __device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, Emit emit) {
   const int tid = threadIdx.x;
+  static_assert(NT >= kCandPad, "");
   if (tid < kCandPad) cand[have + tid] = 0;
   __syncthreads();
   int sh = 0;
@@ -748,12 +775,12 @@ __device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, E
     const int i = i0 + (tid >> sh);
     const cand_t me = i < have ? cand[i] : 0;
     int rank = 0;
-    for (int j = sub; j < have; j += 4 * lanes) {
-      cand_t o[4];
+    for (int j = sub; j < have; j += 8 * lanes) {
+      cand_t o[8];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = cand[j + q * lanes];      // past the end: 0, better than nothing
+      for (int q = 0; q < 8; ++q) o[q] = cand[j + q * lanes];      // past the end: 0, better than nothing
 #pragma unroll
-      for (int q = 0; q < 4; ++q) rank += o[q] > me ? 1 : 0;
+      for (int q = 0; q < 8; ++q) rank += o[q] > me ? 1 : 0;
     }
     if (sh >= 1) rank += (int)dpp_move_u<0xB1>((uint32_t)rank);
     if (sh >= 2) rank += (int)dpp_move_u<0x4E>((uint32_t)rank);
@@ -765,29 +792,43 @@ __device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, E
 
 // The selection's result goes through `emit(rank, key, index)`.
 //
-// Every thread knows the largest value of each of its slot groups.  tau, at most the k-th largest of the threads' largest
-// values (256 of them), is a lower bound of the k-th largest element, so only groups whose largest value reaches tau hold
+// Every thread knows the largest value of each of its slot groups.  tau, at most the k-th largest of the largest values of
+// 256 threads (or sets of threads), is a lower bound of the k-th largest element, so only groups whose largest value reaches tau hold
 // any of the k: these are listed, read again with a slot per thread, and the elements that reach tau - little more than k
 // in an ordinary row - are ranked by counting.  Rows with more candidates than fit (many equal values) take the
 // ordered scan below, and in the worst case one pass over the listed groups per rank.
-template <int DT, int VEC, typename Emit>
-__device__ void block_top(TopShared& sh, const char* p, int V, int n, int s0, int s1, int gsz, int k, float m, float tmax, Emit emit) {
-  constexpr int NT = kRowThreads;
+template <int DT, int VEC, int NT, typename Emit>
+__device__ void block_top(TopShared<NT>& sh, const char* p, int V, int n, int s0, int s1, int gsz, int k, float m, float tmax,
+                          Emit emit) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
   if (tid == 0) sh.count = sh.groups = 0;
   sh.tmax[tid] = tmax;
   __syncthreads();
-  uint32_t g[NT / 64];
+  if (tid < 64) {          // one wavefront searches: the others would only contend with it
+    uint32_t g[kMaxima];
 #pragma unroll
-  for (int w = 0; w < NT / 64; ++w) g[w] = order_key(sh.tmax[64 * w + lane]);
-  uint32_t tau = lower_bound_of<DT, NT / 64>(g, order_key(m), k);
-  if (tau <= kKeyMinusInf) tau = kKeyMinusInf + 1;   // -inf is no alternative
+    for (int w = 0; w < kMaxima; ++w) {
+      float t = sh.tmax[64 * w + lane];
+#pragma unroll
+      for (int j = kMaxima; j < NT / 64; j += kMaxima) t = fmaxf(t, sh.tmax[64 * (w + j) + lane]);
+      g[w] = order_key(t);
+    }
+    const uint32_t t = lower_bound_of<DT, kMaxima>(g, order_key(m), k);
+    if (lane == 0) sh.tau = t <= kKeyMinusInf ? kKeyMinusInf + 1 : t;      // -inf is no alternative
+  }
+  uint32_t gk[kGroups];
+#pragma unroll
+  for (int q = 0; q < kGroups; ++q) gk[q] = order_key(q < groups ? sh.gm[q][tid] : -INFINITY);
+  __syncthreads();
+  uint32_t tau = sh.tau;
   // the groups with a value that reaches `lowest`, in sh.list
   auto list_groups = [&](uint32_t lowest) {
-    if (order_key(tmax) >= lowest)
-      for (int q = 0; q < groups; ++q)
-        if (order_key(sh.gm[q][tid]) >= lowest) sh.list[atomicAdd(&sh.groups, 1)] = (uint16_t)(q * NT + tid);
+    if (order_key(tmax) >= lowest) {
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q)
+        if (gk[q] >= lowest) sh.list[atomicAdd(&sh.groups, 1)] = (uint16_t)(q * NT + tid);
+    }
     __syncthreads();
   };
   // f(keys that reach `lowest`, index of the slot's first element, bits of those elements) for the listed groups
@@ -831,16 +872,24 @@ __device__ void block_top(TopShared& sh, const char* p, int V, int n, int s0, in
   } else {
     // many values reach tau: make it the key of the k-th largest of the threads' values itself (where k threads have
     // one), so that those equal to it can be told from those above
+    uint32_t g[kMaxima];
+#pragma unroll
+    for (int w = 0; w < kMaxima; ++w) {
+      float t = sh.tmax[64 * w + lane];
+#pragma unroll
+      for (int j = kMaxima; j < NT / 64; j += kMaxima) t = fmaxf(t, sh.tmax[64 * (w + j) + lane]);
+      g[w] = order_key(t);
+    }
     auto reach = [&](uint32_t t) {
       int c = 0;
 #pragma unroll
-      for (int w = 0; w < NT / 64; ++w) c += __popcll(__ballot(g[w] >= t));
+      for (int w = 0; w < kMaxima; ++w) c += __popcll(__ballot(g[w] >= t));
       return c;
     };
     for (uint32_t t = tau; reach(t) >= k;) {       // the next of the threads' values, as long as k reach it
       uint32_t next = 0xffffffffu;
 #pragma unroll
-      for (int w = 0; w < NT / 64; ++w) next = (g[w] >= t && g[w] < next) ? g[w] : next;
+      for (int w = 0; w < kMaxima; ++w) next = (g[w] >= t && g[w] < next) ? g[w] : next;
       next = ~gmax_u<64>(~next);
       if (reach(next) < k) break;
       tau = next;
@@ -891,19 +940,19 @@ __device__ void block_top(TopShared& sh, const char* p, int V, int n, int s0, in
       }
     } else {
       // one rank per pass: the best (key, lower index) after the last one
-      unsigned long long last = ~0ull;
+      cand_t last = ~0ull;
       for (done = 0; done < k; ++done) {
-        unsigned long long best = 0;
+        cand_t best = 0;
         each_slot(above, [&](const uint32_t* key, int b, uint32_t bits) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const unsigned long long o = ((unsigned long long)key[e] << 32) | (uint32_t)~(b + e);
+            const cand_t o = candidate(key[e], (uint32_t)(b + e));
             if (((bits >> e) & 1u) && o < last && o > best) best = o;
           }
         });
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
-          const unsigned long long o = __shfl_xor(best, off);
+          const cand_t o = __shfl_xor(best, off);
           best = o > best ? o : best;
         }
         __syncthreads();
@@ -920,12 +969,13 @@ __device__ void block_top(TopShared& sh, const char* p, int V, int n, int s0, in
 }
 
 // One workgroup per row (or per part of a row): every element is read once, kUnroll 16-byte slots in flight per thread.
-template <int DT, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
-  constexpr int NT = kRowThreads, VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
-  __shared__ BlockRed<NT> red;
-  __shared__ int holder;
-  __shared__ typename std::conditional<TOP, TopShared, int>::type top_sh;
+// Four wavefronts where there are rows or parts enough to fill the chip (several workgroups a compute unit hide each
+// other's joins), sixteen where there are few.
+template <int DT, bool ENT, bool TOP, int NT>
+__global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
+  constexpr int VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
+  __shared__ JoinShared<NT> join;
+  __shared__ typename std::conditional<TOP, TopShared<NT>, int>::type top_sh;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x - (int)(row * a.parts);
@@ -936,7 +986,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
   }
   const int n = row_size(a.r, row), V = a.r.V;
   const int ns = (n + VEC - 1) / VEC;
-  const int per = ((ns + a.parts - 1) / a.parts + 63) & ~63;      // whole wavefronts of slots
+  const int per = ((ns + a.parts - 1) / a.parts + 15) & ~15;      // equal to 16 slots
   const int s0 = part * per < ns ? part * per : ns, s1 = s0 + per < ns ? s0 + per : ns;
   const char* p = a.r.x + row * a.r.ld * ES;
   int gsz = (s1 - s0 + NT * kGroups - 1) / (NT * kGroups);    // slots per group of the selection
@@ -944,35 +994,44 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
   Online on;
   float gmx = -INFINITY;
   int in_group = 0, group = 0;
-  for (int s = s0 + tid; s < s1; s += NT * kUnroll) {
-    float v[kUnroll * VEC];
+  // IN slots in flight per thread, kUnroll at a time through the sums
+  constexpr int IN = NT == kWideThreads ? 2 * kUnroll : kUnroll;
+  for (int sb = s0 + tid; sb < s1; sb += NT * IN) {
+    Raw16 raw[IN];
 #pragma unroll
-    for (int q = 0; q < kUnroll; ++q) {
-      const int sq = s + q * NT;
-      const int b = slot_base<VEC>(sq < s1 ? sq : s, V);
-      slot_load<DT, VEC>(p, b, v + q * VEC);
+    for (int q = 0; q < IN; ++q) {
+      const int sq = sb + q * NT;
+      raw[q] = *(const Raw16*)(p + (int64_t)slot_base<VEC>(sq < s1 ? sq : sb, V) * ES);
     }
 #pragma unroll
-    for (int q = 0; q < kUnroll; ++q) {
-      const int sq = s + q * NT;
-      if (sq * VEC + VEC > n || sq >= s1) {       // the row's last slot, and past the end
-        const int b = slot_base<VEC>(sq < s1 ? sq : s, V);
+    for (int h = 0; h < IN; h += kUnroll) {
+      const int s = sb + h * NT;
+      float v[kUnroll * VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (sq >= s1 || b + e < sq * VEC || b + e >= n) v[q * VEC + e] = -INFINITY;
+      for (int q = 0; q < kUnroll; ++q) {
+        Elem<DT>::unpack(raw[h + q], v + q * VEC);
+        const int sq = s + q * NT;
+        if (sq * VEC + VEC > n || sq >= s1) {       // the row's last slot, and past the end
+          const int b = slot_base<VEC>(sq < s1 ? sq : sb, V);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (sq >= s1 || b + e < sq * VEC || b + e >= n) v[q * VEC + e] = -INFINITY;
+        }
       }
-    }
-    const float mx = max_of<kUnroll * VEC>(v, -INFINITY);
-    if constexpr (TOP) {
-      gmx = max3(mx, gmx, gmx);
-      in_group += kUnroll;
-      if (in_group == gsz) {
-        top_sh.gm[group++][tid] = gmx;
-        gmx = -INFINITY;
-        in_group = 0;
+      const float mx = max_of<kUnroll * VEC>(v, -INFINITY);
+      if constexpr (TOP) {
+        if (s < s1) {
+          gmx = max3(mx, gmx, gmx);
+          in_group += kUnroll;
+          if (in_group == gsz) {
+            top_sh.gm[group++][tid] = gmx;
+            gmx = -INFINITY;
+            in_group = 0;
+          }
+        }
       }
+      on.template add<kUnroll * VEC, ENT>(v, mx, a.c);
     }
-    on.template add<kUnroll * VEC, ENT>(v, mx, a.c);
   }
   if constexpr (TOP) {
     const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
@@ -982,7 +1041,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
     }
   }
   float m, r, u;
-  block_join<NT, ENT>(on, a.c, red, &holder, m, r, u, [&](int h, float ref) {
+  block_join<NT, ENT>(on, a.c, join, m, r, u, [&](int h, float ref) {
     float sum = 0.f;
     for (int s = s0 + h + NT * tid; s < s1; s += NT * NT) {
       float v[VEC];
@@ -999,7 +1058,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
     if (tid == 0) a.part[row * a.parts + part] = f32x4{m, r, u, 0.f};
     if constexpr (TOP) {
       uint2* o = a.part_top + (row * a.parts + part) * a.top;
-      block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m,
+      block_top<DT, VEC, NT>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m,
                          [&](int rank, uint32_t key, int i) { o[rank] = make_uint2(key, (uint32_t)i); });
     }
     return;
@@ -1026,25 +1085,19 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_fwd_row(Fwd a) {
       }
       return;
     }
-    block_top<DT, VEC>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m, [&](int rank, uint32_t key, int i) {
+    block_top<DT, VEC, NT>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m, [&](int rank, uint32_t key, int i) {
       a.top_idx[row * a.top + rank] = i;
       a.top_lp[row * a.top + rank] = i < 0 ? -INFINITY : (key_value(key) - m) - logs;
     });
   }
 }
 
-// (m, r, u) of a row from its parts (one wavefront, a lane per part)
+// (m, r, u) of a row from its parts (every wavefront, a lane per part)
 __device__ __forceinline__ void join_parts(const f32x4* part, int parts, float c, float& m, float& r, float& u) {
   const int lane = threadIdx.x & 63;
   const f32x4 me = lane < parts ? part[lane] : f32x4{-INFINITY, -1.f, 0.f, 0.f};
-  m = gmax<64>(me[0]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  const float shift = fmaxf((me[0] - ref) * c, kClampD), f = exp2_hw(shift);
-  const bool holds = me[0] == m && m != -INFINITY;
-  float a = holds ? me[1] : f * (1.f + me[1]);
-  const float b = f * (me[2] - (1.f + me[1]) * shift);
-  r = gsum<64>(a) + (gsum<64>(holds ? 1.f : 0.f) - 1.f);
-  u = gsum<64>(b);
+  m = me[0], r = me[1], u = me[2];
+  join_sets<64>(m, r, u, c);
 }
 
 // The parts' ordered lists hold parts * k candidates.  If j = ceil(k / parts) of every part reach tau, k elements do: tau
@@ -1244,8 +1297,8 @@ template <int DT, int NT, int NV>
 __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
   constexpr int VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
   __shared__ BlockRed<NT> red;
+  __shared__ JoinShared<NT> join;
   __shared__ SparseShared sp;
-  __shared__ int holder;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int V = a.r.V, ns = (V + VEC - 1) / VEC;
@@ -1307,7 +1360,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
   }
   asm volatile("" : "+v"(on.s));        // summed here, not where it is used
   float m, r, u;
-  block_join<NT, false>(on, a.t.c, red, &holder, m, r, u, [&](int h, float ref) {
+  block_join<NT, false>(on, a.t.c, join, m, r, u, [&](int h, float ref) {
     float sum = 0.f;
     if (h == tid) {
 #pragma unroll
@@ -1511,9 +1564,14 @@ void by_type(int dt, F f) {
   else f(std::integral_constant<int, DMV_F16>());
 }
 
-// Workgroups per long row: enough to occupy the chip, but at least one full round of loads (kUnroll slots per thread) each.
+// Few rows: sixteen wavefronts to each, where four would have more than one round of loads.
+bool wide_rows(int64_t groups, int V, int dt) { return groups <= 256 && V > kRowThreads * kUnroll * vec_elems(dt); }
+
+// Workgroups per long row: one as long as its sixteen wavefronts need few rounds of loads (a join is another launch),
+// beyond that enough to occupy the chip.
 int parts_of(int64_t rows, int V, int dt) {
   const int64_t rounds = ((int64_t)V + (int64_t)kChunkSlots * vec_elems(dt) - 1) / ((int64_t)kChunkSlots * vec_elems(dt));
+  if (rounds <= 16) return 1;
   int64_t parts = (1024 + rows - 1) / rows;
   if (parts > rounds) parts = rounds;
   if (parts > kMaxParts) parts = kMaxParts;
@@ -1526,16 +1584,21 @@ bool row_fits(int64_t rows, int V, int dt) { return rows >= kRowMinRows && row_s
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
+template <int DT, int NT>
+void launch_fwd_rows_by(const Fwd& a, bool entropy, hipStream_t st) {
+  const dim3 grid((unsigned)(a.r.rows * a.parts)), block(NT);
+  if (a.top) {
+    if (entropy) k_cat_fwd_row<DT, true, true, NT><<<grid, block, 0, st>>>(a);
+    else k_cat_fwd_row<DT, false, true, NT><<<grid, block, 0, st>>>(a);
+  } else {
+    if (entropy) k_cat_fwd_row<DT, true, false, NT><<<grid, block, 0, st>>>(a);
+    else k_cat_fwd_row<DT, false, false, NT><<<grid, block, 0, st>>>(a);
+  }
+}
 template <int DT>
 void launch_fwd_rows(const Fwd& a, bool entropy, hipStream_t st) {
-  const dim3 grid((unsigned)(a.r.rows * a.parts)), block(kRowThreads);
-  if (a.top) {
-    if (entropy) k_cat_fwd_row<DT, true, true><<<grid, block, 0, st>>>(a);
-    else k_cat_fwd_row<DT, false, true><<<grid, block, 0, st>>>(a);
-  } else {
-    if (entropy) k_cat_fwd_row<DT, true, false><<<grid, block, 0, st>>>(a);
-    else k_cat_fwd_row<DT, false, false><<<grid, block, 0, st>>>(a);
-  }
+  if (wide_rows(a.r.rows * a.parts, a.r.V / a.parts, DT)) launch_fwd_rows_by<DT, kWideThreads>(a, entropy, st);
+  else launch_fwd_rows_by<DT, kRowThreads>(a, entropy, st);
 }
 
 template <int DT>
@@ -1699,7 +1762,7 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
     const int64_t items = r->rows * a.chunks;
     by_type(r->dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
-      k_cat_fwd_row<DT, false, false><<<(unsigned)(r->rows * a.parts), kRowThreads, 0, st>>>(f);
+      launch_fwd_rows<DT>(f, false, st);
       k_cat_distill_join<DT><<<(unsigned)r->rows, kRowThreads, 0, st>>>(a);
       if (a.d) k_cat_distill_chunk<DT><<<(unsigned)(items < 8192 ? items : 8192), kRowThreads, 0, st>>>(a);
     });
