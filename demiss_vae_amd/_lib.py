@@ -18,7 +18,7 @@ GEN = {"normal": 0, "normal_with_eps": 1, "bern": 2, "bern_m1_p1": 3}
 Q_OWN, Q_STRATIFIED, Q_IMPUTATION = 0, 1, 2
 BOUND_LSE, BOUND_WEIGHTED, BOUND_PER_COMPONENT, TERMS_ONLY = 0, 1, 2, -1
 CAT_DTYPE = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
-CAT_MAX_TOP, CAT_MAX_TEACHER, CAT_SHORT_ROW = 64, 256, 1024
+CAT_MAX_TOP, CAT_MAX_TEACHER, CAT_SHORT_ROW = 64, 256, 2048
 E_BADARG, E_UNSUPPORTED, E_WORKSPACE = -1, -2, -3
 
 

@@ -121,6 +121,15 @@ __device__ __forceinline__ float max_of(const float* v, float m) {
   return m;
 }
 
+// log(1 + r), r >= 0 (or NaN), to a few ulp of itself: a series below 2^-6, else log u r / (u - 1) with u = fl(1 + r), in
+// which the rounding of u cancels; the reciprocal unit's ulp is all that is added
+__device__ __forceinline__ float log1p_row(float r) {
+  const float u = 1.f + r;
+  const float far = r < INFINITY ? __logf(u) * (r * __builtin_amdgcn_rcpf(u - 1.f)) : r;
+  const float near = r * (1.f - r * (0.5f - r * (1.f / 3.f - r * (0.25f - r * 0.2f))));
+  return r < 0x1p-6f ? near : far;
+}
+
 __device__ __forceinline__ float exp2_hw(float d) { return __builtin_amdgcn_exp2f(d); }
 
 template <int R>
@@ -159,11 +168,9 @@ struct Rows {
   int64_t x_period, m_period, size_period;
 };
 
-// entry of a per-row array that repeats with `period` rows
+// entry of a per-row array that repeats with `period` rows (there are fewer than 2^31 rows)
 __device__ __forceinline__ int64_t wrap(int64_t row, int64_t period, int64_t rows) {
-  if (period == rows) return row;
-  if ((uint64_t)rows <= 0xffffffffull) return (int64_t)((uint32_t)row % (uint32_t)period);
-  return row % period;
+  return period >= rows ? row : (int64_t)((uint32_t)row % (uint32_t)period);
 }
 __device__ __forceinline__ int row_size(const Rows& a, int64_t row) {
   if (!a.sizes) return a.V;
@@ -276,138 +283,222 @@ struct RowGrad {
 };
 
 // ------------------------------------------------------------------------------------------ short rows
-// L lanes hold a row of up to 16 L elements in registers (SL slots of VEC elements each); 64 / L rows per wavefront.
+// L lanes hold a row of up to 32 L elements in registers (SL slots of VEC elements each); 64 / L rows per wavefront.  What a
+// row costs apart from its elements (addresses, reductions, logarithm, outputs) is as much for 4 lanes as for 64, so L is
+// the smallest that holds the row.
 constexpr int kSmallThreads = 256;
+constexpr int kSmallMax = DMV_CAT_SHORT_ROW;   // their longest row: 64 lanes, 32 elements each
+
+// Candidates of a selection: key in the upper half, ~index in the lower, so that the larger number is the better one.
+typedef unsigned long long cand_t;
+__device__ __forceinline__ cand_t candidate(uint32_t key, uint32_t index) { return ((cand_t)key << 32) | (uint32_t)~index; }
+
+template <int DT, int VEC>
+struct SmallSlot {
+  Raw16 raw;
+  __device__ __forceinline__ void load(const char* p, int base) {
+    raw = *(const Raw16*)(p + (int64_t)base * (int)sizeof(typename Elem<DT>::type));
+  }
+  __device__ __forceinline__ void unpack(float* v) const { Elem<DT>::unpack(raw, v); }
+  __device__ __forceinline__ void pack(const float* v) { Elem<DT>::pack(v, raw); }
+};
+template <int DT>
+struct SmallSlot<DT, 1> {
+  float x;
+  __device__ __forceinline__ void load(const char* p, int base) { x = Elem<DT>::load(p, base); }
+  __device__ __forceinline__ void unpack(float* v) const { v[0] = x; }
+  __device__ __forceinline__ void pack(const float* v) { x = v[0]; }
+};
 
 template <int DT, int VEC, int L, int SL>
 struct SmallRow {
   static constexpr int E = VEC * SL;
-  float v[E];
-  int n, lane;
-  const char* p;
-  // element e of this lane: its index in the row, and whether it counts (each category exactly once, below n)
-  __device__ __forceinline__ int first(int j) const { return (lane + L * j) * VEC; }
-  __device__ __forceinline__ void load(const Rows& a, int64_t row, int lane_, int n_) {
-    lane = lane_;
-    n = n_;
-    p = a.x + row * a.ld * (int64_t)sizeof(typename Elem<DT>::type);
+  SmallSlot<DT, VEC> slot[SL];
+  // (a lane without a slot gets the row's last one)
+  __device__ __forceinline__ void load(const char* p, int V, int lane) {
 #pragma unroll
     for (int j = 0; j < SL; ++j) {
-      if (first(j) < a.V) {
-        slot_load<DT, VEC>(p, slot_base<VEC>(lane + L * j, a.V), v + j * VEC);
-      } else {
+      const int b = (lane + L * j) * VEC;
+      slot[j].load(p, b + VEC <= V ? b : V - VEC);
+    }
+  }
+  // every category once: what is past n, past the row, or shared with the slot before becomes -inf
+  __device__ __forceinline__ void count_once(int V, int n, int lane) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[j * VEC + e] = -INFINITY;
+    for (int j = 0; j < SL; ++j) {
+      const int f = (lane + L * j) * VEC;
+      if (f + VEC > n) {
+        const int b = f + VEC <= V ? f : V - VEC;
+        float v[VEC];
+        slot[j].unpack(v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = (b + e >= f && b + e < n) ? v[e] : -INFINITY;
+        slot[j].pack(v);
       }
     }
   }
-  // the elements that do not count become -inf
-  __device__ __forceinline__ void counted(int V, float* o) const {
+  __device__ __forceinline__ void values(float* o) const {
 #pragma unroll
-    for (int j = 0; j < SL; ++j) {
-      const int b = slot_base<VEC>(lane + L * j, V), f = first(j);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int i = b + e;
-        o[j * VEC + e] = (i >= f && i < n) ? v[j * VEC + e] : -INFINITY;
-      }
-    }
+    for (int j = 0; j < SL; ++j) slot[j].unpack(o + j * VEC);
   }
 };
 
 // (m, r, u) of a row held by L lanes; r < 0: no category of non-zero probability
-template <int L, int E>
-__device__ __forceinline__ void small_stats(const float* o, float c, bool entropy, float& m, float& r, float& u) {
+template <bool ENT, int L, int E>
+__device__ __forceinline__ void small_stats(const float* o, float c, float& m, float& r, float& u) {
   m = gmax<L>(max_of<E>(o, -INFINITY));
   const float ref = m == -INFINITY ? 0.f : m;
+  // in blocks of eight: left alone, the scheduler holds every element's difference and exponential at once
   float s = 0.f, t = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
+    if (e % 8 == 0) __builtin_amdgcn_sched_barrier(0);
     const float d = (o[e] - ref) * c, w = exp2_hw(d);
     s += w;
-    if (entropy) t = fmaf(w, fmaxf(d, kClampD), t);
+    if (ENT) t = fmaf(w, fmaxf(d, kClampD), t);
   }
+  u = ENT ? -gsum<L>(t) : 0.f;
   r = gsum<L>(s) - 1.f;
-  u = entropy ? -gsum<L>(t) : 0.f;
   if (r < kNearCertain && r >= 0.f) {
     s = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += o[e] < m ? exp2_hw((o[e] - m) * c) : 0.f;
+    for (int e = 0; e < E; ++e) {
+      if (e % 8 == 0) __builtin_amdgcn_sched_barrier(0);
+      s += o[e] < m ? exp2_hw((o[e] - m) * c) : 0.f;
+    }
     r = gsum<L>(s);
   }
 }
 
-template <int DT, int VEC, int L, int SL>
-__global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
+// The k largest of a row held by L lanes, through emit(rank, value, index) by any lane; index -1 past the finite values.
+//
+// Few of them (k <= L, 8 or more lanes): the lanes fall into at least k sets; the smallest of the sets' largest values is a
+// lower bound of the k-th largest value, which about k ln k elements reach.  Those go to the group's list in LDS and are
+// ranked by counting.  Otherwise, or when the list is too short for them, one rank at a time.
+constexpr int kSmallList = 8;            // list entries per lane
+template <int L>
+__device__ __forceinline__ float sets_min(float mx, int k) {
+  // sets of L / S lanes, S >= k a power of two: the largest within, the smallest across
+  auto step = [&](float other, bool across) { mx = across ? fminf(mx, other) : fmaxf(mx, other); };
+  if (L >= 2) step(dpp_move<0xB1>(mx), k > L / 2);
+  if (L >= 4) step(dpp_move<0x4E>(mx), k > L / 4);
+  if (L >= 8) step(dpp_move<0x141>(mx), k > L / 8);
+  if (L >= 16) step(dpp_move<0x140>(mx), k > L / 16);
+  if (L >= 32) step(__shfl_xor(mx, 16), k > L / 32);
+  if (L >= 64) step(__shfl_xor(mx, 32), k > L / 64);
+  return mx;
+}
+// lanes of one wavefront that read what others of it wrote: in order without a wait
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+template <int DT, int VEC, int L, int SL, typename Emit>
+__device__ __forceinline__ void small_top(const float* o, const char* p, int V, int lane, int k, cand_t* list, int* count, Emit emit) {
   constexpr int E = VEC * SL;
-  const int lane = threadIdx.x & (L - 1);
-  const int64_t row = (int64_t)blockIdx.x * (kSmallThreads / L) + threadIdx.x / L;
-  if (row >= a.r.rows) return;
-  const bool seen = row_seen(a.r, row);
-  if (!seen && !a.entropy && !a.top) {
-    if (lane == 0 && a.log_prob) a.log_prob[row] = 0.f;
-    return;
-  }
-  const int n = row_size(a.r, row);
-  SmallRow<DT, VEC, L, SL> x;
-  x.load(a.r, row, lane, n);
-  int64_t X = -1;
-  float xX = -INFINITY;
-  if (a.log_prob && seen) {
-    X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
-    if (X >= 0 && X < n) xX = Elem<DT>::load(x.p, X);
-  }
-  float o[E], m, r, u;
-  x.counted(a.r.V, o);
-  small_stats<L, E>(o, a.c, a.entropy != nullptr, m, r, u);
-  const bool empty = m == -INFINITY && !(r != r);
-  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
-  const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
-  if (lane == 0) {
-    if (a.log_prob) {
-      float lp = 0.f;
-      if (seen) lp = (X < 0 || X >= n) ? NAN : (empty ? -INFINITY : (xX - m) - logs);
-      a.log_prob[row] = lp;
+  auto index = [&](int j, int e) { return slot_base<VEC>(lane + L * j, V) + e; };
+  if (L >= 8 && k <= L) {
+    const float bound = fmaxf(sets_min<L>(max_of<E>(o, -INFINITY), k), -3.402823466e38f);      // -inf is no alternative
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = E - 1; i >= 0; --i) bits = bits + bits + (o[i] >= bound ? 1u : 0u);
+    if (lane == 0) *count = 0;
+    wave_sync();
+    if (bits) {
+      int at = atomicAdd(count, __popc(bits));
+      do {          // few: their values are read again rather than picked from registers
+        const int i = __ffs(bits) - 1;
+        bits &= bits - 1;
+        const int at_v = index(i / VEC, i % VEC);
+        if (at < kSmallList * L) list[at] = candidate(order_key(Elem<DT>::load(p, at_v)), (uint32_t)at_v);
+        ++at;
+      } while (bits);
     }
-    if (a.entropy) a.entropy[row] = H;
-    if (a.stats) a.stats[row] = f32x4{m, inv_s, logs, H};
+    wave_sync();
+    const int have = *count;
+    if (have <= kSmallList * L) {
+      for (int i = lane; i < have; i += L) {
+        const cand_t me = list[i];
+        int rank = 0;
+        for (int j = 0; j < have; ++j) rank += list[j] > me ? 1 : 0;
+        if (rank < k) emit(rank, key_value((uint32_t)(me >> 32)), (int)~(uint32_t)me);
+      }
+      for (int j = have + lane; j < k; j += L) emit(j, -INFINITY, -1);
+      return;
+    }
   }
-  if (a.top) {
-    const bool bad = logs != logs;
-    uint32_t k[E];
+  // one rank at a time: what has been ranked is all that is better than the last one
+  float last = INFINITY;
+  int last_at = -1;
+  for (int t = 0; t < k; ++t) {
+    float best = -INFINITY;
+    int at = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < SL; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float w = o[j * VEC + e];
-        k[j * VEC + e] = (w > -INFINITY) ? order_key(w) : 0u;
-      }
-    for (int t = 0; t < a.top; ++t) {
-      uint32_t best = 0;
-      int at = 0x7fffffff;
-#pragma unroll
-      for (int j = 0; j < SL; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const uint32_t w = k[j * VEC + e];
-          if (w > best) {
-            best = w;
-            at = slot_base<VEC>(lane + L * j, a.r.V) + e;
-          }
+        const float x = o[j * VEC + e];
+        if ((x < last || (x == last && index(j, e) > last_at)) && x > best) {
+          best = x;
+          at = index(j, e);
         }
-      const uint32_t top = gmax_u<L>(best);
-      const uint32_t low = ~gmax_u<L>(best == top ? ~(uint32_t)at : 0u);   // lowest index among the equal ones
-#pragma unroll
-      for (int j = 0; j < SL; ++j)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (slot_base<VEC>(lane + L * j, a.r.V) + e == (int)low) k[j * VEC + e] = 0u;
-      if (lane == (t & (L - 1))) {
-        const int64_t at_out = row * a.top + t;
-        const bool none = top == 0u || bad;
-        a.top_idx[at_out] = none ? -1 : (int64_t)low;
-        a.top_lp[at_out] = bad ? NAN : (none ? -INFINITY : (key_value(top) - m) - logs);
       }
+    const float top = gmax<L>(best);
+    const uint32_t low = ~gmax_u<L>(best == top ? ~(uint32_t)at : 0u);   // lowest index among the equal ones
+    const bool none = top == -INFINITY;
+    if (lane == (t & (L - 1))) emit(t, top, none ? -1 : (int)low);
+    last = top;
+    last_at = (int)low;
+  }
+}
+
+template <int DT, int VEC, int L, int SL, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
+  constexpr int E = VEC * SL, NG = kSmallThreads / L, ES = sizeof(typename Elem<DT>::type);
+  __shared__ cand_t lists[TOP && L >= 8 ? NG : 1][TOP && L >= 8 ? kSmallList * L : 1];
+  __shared__ int counts[NG];
+  const int lane = threadIdx.x & (L - 1), V = a.r.V;
+  const int row = blockIdx.x * NG + threadIdx.x / L;          // (rows * 16 bytes fit 32 bits)
+  if (row >= (int)a.r.rows) return;
+  const bool seen = row_seen(a.r, row);
+  if (!TOP && !ENT && !seen) {
+    if (lane == 0) a.log_prob[(uint32_t)row] = 0.f;
+    return;
+  }
+  const int n = row_size(a.r, row);
+  const char* p = a.r.x + row * a.r.ld * ES;
+  SmallRow<DT, VEC, L, SL> x;
+  x.load(p, V, lane);
+  bool given = false;
+  float xX = 0.f;
+  if (a.log_prob && seen) {
+    const int64_t X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
+    given = X >= 0 && X < n;
+    if (given) xX = Elem<DT>::load(p, X);
+  }
+  float o[E], m, r, u;
+  x.count_once(V, n, lane);
+  x.values(o);
+  small_stats<ENT, L, E>(o, a.c, m, r, u);
+  const bool empty = m == -INFINITY && !(r != r);
+  const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
+  const float H = empty ? 0.f : fmaf(kLn2 * u, inv_s, logs);
+  if (lane == 0) {
+    if (a.log_prob) a.log_prob[(uint32_t)row] = !seen ? 0.f : (!given ? NAN : (empty ? -INFINITY : (xX - m) - logs));
+    if (ENT) a.entropy[(uint32_t)row] = H;
+    if (a.stats) a.stats[(uint32_t)row] = f32x4{m, inv_s, logs, H};
+  }
+  if constexpr (TOP) {
+    float* lp = a.top_lp + (int64_t)row * a.top;
+    int64_t* idx = a.top_idx + (int64_t)row * a.top;
+    if (logs != logs) {
+      for (int j = lane; j < a.top; j += L) lp[j] = NAN, idx[j] = -1;
+    } else {
+      const int g = threadIdx.x / L;
+      small_top<DT, VEC, L, SL>(o, p, V, lane, a.top, lists[TOP && L >= 8 ? g : 0], &counts[g], [&](int rank, float v, int i) {
+        idx[rank] = i;
+        lp[rank] = i < 0 ? -INFINITY : (v - m) - logs;
+      });
     }
   }
 }
@@ -450,6 +541,7 @@ __device__ __forceinline__ RowGrad row_grad(const Bwd& a, int64_t row, int lane,
 
 template <int DT, int VEC, int L, int SL>
 __global__ void __launch_bounds__(kSmallThreads) k_cat_bwd_small(Bwd a) {
+  constexpr int ES = sizeof(typename Elem<DT>::type);
   const int lane = threadIdx.x & (L - 1);
   const int64_t row = (int64_t)blockIdx.x * (kSmallThreads / L) + threadIdx.x / L;
   if (row >= a.r.rows) return;
@@ -457,28 +549,36 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_bwd_small(Bwd a) {
   int64_t X;
   float gl;
   const RowGrad g = row_grad<L>(a, row, lane, n, X, gl);
-  char* out = (char*)a.d + row * a.ld_d * (int64_t)sizeof(typename Elem<DT>::type);
+  const char* p = a.r.x + row * a.r.ld * ES;
+  char* out = (char*)a.d + row * a.ld_d * ES;
   const bool live = (g.S != 0.f || g.gh != 0.f || a.g_top) && g.inv_s != 0.f;
   SmallRow<DT, VEC, L, SL> x;
-  if (live) x.load(a.r, row, lane, n);
+  if (live) x.load(p, V, lane);
 #pragma unroll
   for (int j = 0; j < SL; ++j) {
-    const int f = (lane + L * j) * VEC;
-    if (f >= V) continue;
-    const int b = slot_base<VEC>(lane + L * j, V);
+    const int s = lane + L * j;
+    if (s * VEC >= V) continue;
+    const int b = slot_base<VEC>(s, V);
     float o[VEC];
+    if (live) {
+      float v[VEC];
+      x.slot[j].unpack(v);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = (live && b + e < n) ? g.dense(x.v[j * VEC + e]) : 0.f;
+      for (int e = 0; e < VEC; ++e) o[e] = b + e < n ? g.dense(v[e]) : 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = 0.f;
+    }
     slot_store<DT, VEC>(out, b, o);
   }
   if (!live) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // the dense part before the few categories written again
-  __builtin_amdgcn_wave_barrier();
+  // the dense part before the few categories written again: stores of one wavefront stay in order
+  wave_sync();
   const int entries = 1 + (a.g_top ? a.top : 0);
   for (int j = lane; j < entries; j += L) {
     const int64_t v = j == 0 ? X : a.top_idx[row * a.top + j - 1];
     if (v < 0 || v >= n) continue;
-    Elem<DT>::store(out, v, g.at(Elem<DT>::load(x.p, v), own_share(a, row, v, X, gl)));
+    Elem<DT>::store(out, v, g.at(Elem<DT>::load(p, v), own_share(a, row, v, X, gl)));
   }
 }
 
@@ -487,15 +587,6 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_bwd_small(Bwd a) {
 // themselves.  An index past the row's categories, or a logit that is NaN or +inf, makes the row's loss and gradient NaN.
 __device__ __forceinline__ bool entry_counts(float t, int64_t i) { return i >= 0 && t != -INFINITY; }
 
-template <int DT>
-struct Student {
-  float m, inv_s, logs, c, inv_T;
-  const char* p;
-  // log q of category v (any rounding of the sum near 1 is already in logs)
-  __device__ __forceinline__ float log_q(int64_t v) const { return (Elem<DT>::load(p, v) - m) * inv_T - logs; }
-  __device__ __forceinline__ float q(float x) const { return exp2_hw((x - m) * c) * inv_s; }
-};
-
 // q - p without its cancellation
 __device__ __forceinline__ float q_minus_p(float lq, float p) {
   const float q = expf(lq);
@@ -503,97 +594,127 @@ __device__ __forceinline__ float q_minus_p(float lq, float p) {
   return q - p;
 }
 
+// A teacher's entry in LDS: probability, log q of its category, category (-1: empty).
+struct Entry {
+  float p, lq;
+  int i;
+};
+constexpr int kFewEntries = 16;       // up to here a category given twice is looked for entry by entry
+
 template <int DT, int VEC, int L, int SL>
 __global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
-  constexpr int E = VEC * SL;
+  constexpr int E = VEC * SL, NG = kSmallThreads / L, ES = sizeof(typename Elem<DT>::type), WORDS = E * L / 32;
   __shared__ double sums[kSmallThreads / 64];
+  __shared__ uint32_t given[NG][WORDS];
+  extern __shared__ Entry entries[];    // [NG][k]
   const float gs = a.gscale ? *a.gscale : 1.f;
   if (a.unless_one && gs == 1.f) return;
-  const int lane = threadIdx.x & (L - 1);
-  const int64_t row = (int64_t)blockIdx.x * (kSmallThreads / L) + threadIdx.x / L;
-  float kl = 0.f, w = 0.f;
-  if (row < a.r.rows) {
-    const int n = row_size(a.r, row), V = a.r.V, K = a.t.k;
-    w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
+  const int lane = threadIdx.x & (L - 1), V = a.r.V, K = a.t.k, g = threadIdx.x / L;
+  const int row = blockIdx.x * NG + g;
+  double part = 0.0;
+  const float w = row >= (int)a.r.rows ? 0.f : (a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f);
+  float kl = 0.f;
+  if (w != 0.f) {
+    const char* p = a.r.x + row * a.r.ld * ES;
     SmallRow<DT, VEC, L, SL> x;
-    Student<DT> st;
-    bool any = false, bad = false, empty = true;
-    float tm = -INFINITY, t_logs = 0.f;
+    x.load(p, V, lane);
+    const int n = row_size(a.r, row);
+    Entry* own = entries + g * K;
     const int64_t t0 = wrap(row, a.t.t_period, a.r.rows) * K;
-    if (w != 0.f) {
-      x.load(a.r, row, lane, n);
-      for (int j = lane; j < K; j += L) {
-        const int64_t i = a.t.idx[t0 + j];
-        const float t = teacher_logit(a.t, t0 + j);
-        if (!entry_counts(t, i)) continue;
-        any = true;
-        bad = bad || i >= n || !(t < INFINITY);
-        tm = fmaxf(tm, t);
-      }
-      tm = gmax<L>(tm);
-      any = gmax<L>(any ? 1.f : 0.f) > 0.f;
-      bad = gmax<L>(bad ? 1.f : 0.f) > 0.f;
-      float s = 0.f, held = 0.f;
-      for (int j = lane; j < K; j += L) {
-        const int64_t i = a.t.idx[t0 + j];
-        const float t = teacher_logit(a.t, t0 + j);
-        if (!entry_counts(t, i)) continue;
-        if (t == tm) held += 1.f;
-        else s += exp2_hw((t - tm) * a.t.c);
-      }
-      t_logs = log1pf(gsum<L>(s) + (gsum<L>(held) - 1.f));
-      float o[E], m, r, u;
-      x.counted(V, o);
-      small_stats<L, E>(o, a.t.c, false, m, r, u);
-      empty = m == -INFINITY && !(r != r);
-      st.m = m, st.c = a.t.c, st.inv_T = a.t.inv_T, st.p = x.p;
-      st.logs = empty ? 0.f : log1pf(r);
-      st.inv_s = empty ? 0.f : 1.f / (1.f + r);
-      if (lane == 0 && a.stats) a.stats[row] = f32x4{st.m, st.inv_s, st.logs, 0.f};
-      if (any && !bad && !empty) {
-        for (int j = lane; j < K; j += L) {
-          const int64_t i = a.t.idx[t0 + j];
-          const float t = teacher_logit(a.t, t0 + j);
-          if (!entry_counts(t, i)) continue;
-          const float lp = (t - tm) * a.t.inv_T - t_logs, p = expf(lp);
-          if (p > 0.f) kl += p * (lp - st.log_q(i));
-        }
-      }
-      kl = gsum<L>(kl);
-      if (any && empty) kl = INFINITY;
-      if (bad) kl = NAN;
+    float tm = -INFINITY;
+    uint32_t flags = 0;                 // 1: an entry counts, 2: one that cannot be
+    for (int j = lane; j < K; j += L) {
+      const int64_t i = a.t.idx[t0 + j];
+      const float t = teacher_logit(a.t, t0 + j);
+      const bool counts = entry_counts(t, i), bad = counts && (i >= n || !(t < INFINITY));
+      flags |= (counts ? 1u : 0u) | (bad ? 2u : 0u);
+      if (counts) tm = fmaxf(tm, t);
+      own[j] = Entry{t, counts && !bad ? Elem<DT>::load(p, i) : 0.f, counts && !bad ? (int)i : -1};
     }
-    if (lane == 0 && a.per_row) a.per_row[row] = kl;
+    tm = gmax<L>(tm);
+    flags = gmax_u<L>(flags);
+    const bool any = flags != 0u, bad = flags >= 2u;
+    float o[E], m, r, u;
+    x.count_once(V, n, lane);
+    x.values(o);
+    small_stats<false, L, E>(o, a.t.c, m, r, u);
+    const bool empty = m == -INFINITY && !(r != r);
+    const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
+    const bool live = any && !empty;
+    if (live && !bad) {
+      float s = 0.f, held = 0.f;
+      for (int j = lane; j < K; j += L)
+        if (own[j].i >= 0) {
+          if (own[j].p == tm) held += 1.f;
+          else s += exp2_hw((own[j].p - tm) * a.t.c);
+        }
+      const float t_logs = log1p_row(gsum<L>(s) + (gsum<L>(held) - 1.f));
+      for (int j = lane; j < K; j += L)
+        if (own[j].i >= 0) {
+          const float lp = (own[j].p - tm) * a.t.inv_T - t_logs, q = expf(lp), lq = (own[j].lq - m) * a.t.inv_T - logs;
+          if (q > 0.f) kl += q * (lp - lq);
+          own[j].p = q;
+          own[j].lq = lq;
+        }
+      kl = gsum<L>(kl);
+    }
+    if (any && empty) kl = INFINITY;
+    if (bad) kl = NAN;
+    if (lane == 0) part = (double)w * (double)kl;
     if (a.d) {
-      char* out = (char*)a.d + row * a.ld_d * (int64_t)sizeof(typename Elem<DT>::type);
-      const bool live = w != 0.f && any && !empty;
-      const float scale = bad ? NAN : gs * w * a.t.inv_T;
+      char* out = (char*)a.d + row * a.ld_d * ES;
+      const float scale = bad ? NAN : gs * w * a.t.inv_T, f = live ? scale * inv_s : 0.f;
 #pragma unroll
       for (int j = 0; j < SL; ++j) {
-        const int f = (lane + L * j) * VEC;
-        if (f >= V) continue;
-        const int b = slot_base<VEC>(lane + L * j, V);
-        float g[VEC];
+        const int fst = (lane + L * j) * VEC;
+        if (fst >= V) continue;
+        __builtin_amdgcn_sched_barrier(0);
+        float v[VEC];
+        x.slot[j].unpack(v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = (live && b + e < n) ? scale * st.q(x.v[j * VEC + e]) : 0.f;
-        slot_store<DT, VEC>(out, b, g);
+        for (int e = 0; e < VEC; ++e) v[e] = live ? f * exp2_hw((v[e] - m) * a.t.c) : 0.f;     // (what does not count: 0)
+        if (fst + VEC <= V) slot_store<DT, VEC>(out, fst, v);
+        else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (V - VEC + e >= fst) Elem<DT>::store(out, V - VEC + e, v[e]);
+        }
       }
       if (live && !bad) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-        __builtin_amdgcn_wave_barrier();
+        // A category given more than once has all its entries' probability in each of them.  Whether there is one is told
+        // by a bit per category.
+        bool twice = K <= kFewEntries;
+        if (!twice) {
+          for (int q = lane; q < WORDS; q += L) given[g][q] = 0u;
+          wave_sync();
+          for (int j = lane; j < K; j += L)
+            if (own[j].i >= 0) {
+              const uint32_t bit = 1u << (own[j].i & 31);
+              twice = twice || (atomicOr(&given[g][own[j].i >> 5], bit) & bit) != 0u;
+            }
+          twice = gmax_u<L>(twice ? 1u : 0u) != 0u;
+        }
+        // the dense part before the teacher's categories are written again: stores of one wavefront stay in order
+        wave_sync();
         for (int j = lane; j < K; j += L) {
-          const int64_t i = a.t.idx[t0 + j];
-          if (!entry_counts(teacher_logit(a.t, t0 + j), i)) continue;
-          float p = 0.f;      // the same category may be given more than once
-          for (int h = 0; h < K; ++h)
-            if (a.t.idx[t0 + h] == i) p += expf((teacher_logit(a.t, t0 + h) - tm) * a.t.inv_T - t_logs);
-          Elem<DT>::store(out, i, scale * q_minus_p(st.log_q(i), p));
+          const Entry e = own[j];
+          if (e.i < 0) continue;
+          float sum = e.p;
+          if (twice) {
+            sum = 0.f;
+            for (int h = 0; h < K; ++h) sum += own[h].i == e.i ? own[h].p : 0.f;
+          }
+          Elem<DT>::store(out, e.i, scale * q_minus_p(e.lq, sum));
         }
       }
     }
+  } else if (a.d && row < (int)a.r.rows) {
+    char* out = (char*)a.d + row * a.ld_d * ES;
+    const float z[VEC] = {};
+    for (int sl = lane; sl * VEC < V; sl += L) slot_store<DT, VEC>(out, slot_base<VEC>(sl, V), z);
   }
+  if (lane == 0 && a.per_row && row < (int)a.r.rows) a.per_row[(uint32_t)row] = kl;
   // the workgroup's share of the loss, in a fixed order
-  double part = (lane == 0 && w != 0.f) ? (double)w * (double)kl : 0.0;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) part += __shfl_xor(part, off);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = part;
@@ -716,9 +837,6 @@ constexpr int kUnroll = 4;              // slots in flight per thread
 constexpr int kGroups = 8;              // slot groups whose maxima a thread keeps for the selection
 constexpr int kCand = 512;              // candidates of a selection
 
-// Candidates of a selection: key in the upper half, ~index in the lower, so that the larger number is the better one.
-typedef unsigned long long cand_t;
-__device__ __forceinline__ cand_t candidate(uint32_t key, uint32_t index) { return ((cand_t)key << 32) | (uint32_t)~index; }
 constexpr int kCandPad = 128;
 
 constexpr int kMaxima = 4;              // largest values a lane holds in the search for the bound: 256 in all
@@ -1063,7 +1181,7 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
     }
     return;
   }
-  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
   const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
   if (tid == 0) {
     if (a.log_prob) {
@@ -1116,7 +1234,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_cat_fwd_join(Fwd a) {
   float m, r, u;
   join_parts(a.part + row * a.parts, a.parts, a.c, m, r, u);
   const bool empty = m == -INFINITY && !(r != r);
-  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
   const float H = empty ? 0.f : logs + kLn2 * u * inv_s;
   if (tid == 0) {
     count = 0;
@@ -1261,7 +1379,7 @@ __device__ __forceinline__ TeacherEntry teacher_row(const Teacher& t, int64_t ro
   e.bad = b > 0.f;
   e.any = held > 0.f || e.bad;
   if (counts) {
-    e.lp = (x - tm) * t.inv_T - log1pf(s + (held - 1.f));
+    e.lp = (x - tm) * t.inv_T - log1p_row(s + (held - 1.f));
     e.p = expf(e.lp);
   }
   return e;
@@ -1374,7 +1492,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
     return sum;
   });
   const bool empty = m == -INFINITY && r == -1.f;
-  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
   const float lq = (xi - m) * a.t.inv_T - logs;
   float kl = (te.i >= 0 && te.p > 0.f && !empty) ? te.p * (te.lp - lq) : 0.f, z0 = 0.f, z1 = 0.f;
   if (tid < a.t.k) {
@@ -1432,7 +1550,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_distill_join(Dist a) {
   float m, r, u;
   join_parts(a.part + row * a.parts, a.parts, a.t.c, m, r, u);     // every wavefront does the same
   const bool empty = m == -INFINITY && !(r != r);
-  const float logs = empty ? 0.f : log1pf(r), inv_s = empty ? 0.f : 1.f / (1.f + r);
+  const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
   float kl = (te.i >= 0 && te.p > 0.f && !empty) ? te.p * (te.lp - ((xi - m) * a.t.inv_T - logs)) : 0.f, z0 = 0.f, z1 = 0.f;
   block_sum3<NT>(kl, z0, z1, red);
   if (te.any && empty) kl = INFINITY;
@@ -1521,7 +1639,6 @@ __global__ void __launch_bounds__(kLossThreads) k_cat_loss(const double* part, i
 
 // ------------------------------------------------------------------------------------------ host side
 constexpr int64_t kMaxGrid = 0x7fffffffll;
-constexpr int kSmallMax = DMV_CAT_SHORT_ROW;   // longest row of the register kernels of short rows
 
 int check_rows(const DmvCatRows* r) {
   if (!r || r->rows < 0 || r->V < 1 || r->ld < 0) return DMV_E_BADARG;
@@ -1537,25 +1654,32 @@ Rows rows_of(const DmvCatRows* r) {
   return Rows{(const char*)r->logits, r->ld, r->rows, r->V, r->X, r->M, r->sizes, r->x_period, r->m_period, r->size_period};
 }
 
-// Short rows: `f` gets the tag of the smallest register tile that holds V elements (16 elements a lane; rows shorter
+// Short rows: `f` gets the tag of the smallest register tile that holds V elements (up to 32 elements a lane; rows shorter
 // than a 16-byte slot are read one element at a time).
 template <int DT_, int VEC_, int L_, int SL_>
 struct Tile {
   static constexpr int DT = DT_, VEC = VEC_, L = L_, SL = SL_;
+  static int64_t groups(int64_t rows) { return (rows + kSmallThreads / L - 1) / (kSmallThreads / L); }
 };
 template <int DT, typename F>
 void small_tile(int V, F f) {
-  constexpr int N = Elem<DT>::N, S = 16 / N;
+  constexpr int N = Elem<DT>::N, S = 32 / N;
   const int ns = (V + N - 1) / N;
   if (V < N) return f(Tile<DT, 1, 4, 2>());
   if (ns <= 4) return f(Tile<DT, N, 4, 1>());
   if (ns <= 8) return f(Tile<DT, N, 4, 2>());
-  if constexpr (S == 4)
-    if (ns <= 16) return f(Tile<DT, N, 4, 4>());
+  if (ns <= 16) return f(Tile<DT, N, 4, 4>());
+  if constexpr (S == 8)
+    if (ns <= 32) return f(Tile<DT, N, 4, 8>());
   if (ns <= 8 * S) return f(Tile<DT, N, 8, S>());
   if (ns <= 16 * S) return f(Tile<DT, N, 16, S>());
   if (ns <= 32 * S) return f(Tile<DT, N, 32, S>());
   return f(Tile<DT, N, 64, S>());
+}
+// LDS of a workgroup's teacher entries
+template <typename T>
+size_t small_lds(int k) {
+  return (size_t)(kSmallThreads / T::L) * k * sizeof(Entry);
 }
 template <typename F>
 void by_type(int dt, F f) {
@@ -1637,8 +1761,14 @@ extern "C" int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* ent
     by_type(r->dtype, [&](auto dt) {
       small_tile<decltype(dt)::value>(r->V, [&](auto t) {
         typedef decltype(t) T;
-        k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL>
-            <<<dmv_ceil_div(r->rows, kSmallThreads / T::L), kSmallThreads, 0, st>>>(a);
+        const dim3 grid((unsigned)T::groups(r->rows)), block(kSmallThreads);
+        if (a.top) {
+          if (entropy) k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, true, true><<<grid, block, 0, st>>>(a);
+          else k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, false, true><<<grid, block, 0, st>>>(a);
+        } else {
+          if (entropy) k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, true, false><<<grid, block, 0, st>>>(a);
+          else k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, false, false><<<grid, block, 0, st>>>(a);
+        }
       });
     });
     DMV_HIP_CHECK_LAUNCH();
@@ -1675,8 +1805,7 @@ extern "C" int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats
     by_type(r->dtype, [&](auto dt) {
       small_tile<decltype(dt)::value>(r->V, [&](auto t) {
         typedef decltype(t) T;
-        k_cat_bwd_small<T::DT, T::VEC, T::L, T::SL>
-            <<<dmv_ceil_div(r->rows, kSmallThreads / T::L), kSmallThreads, 0, st>>>(a);
+        k_cat_bwd_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)T::groups(r->rows), kSmallThreads, 0, st>>>(a);
       });
     });
     DMV_HIP_CHECK_LAUNCH();
@@ -1708,7 +1837,7 @@ static int64_t loss_parts(const DmvCatRows* r) {
   int64_t n = r->rows;
   if (r->V <= kSmallMax)
     by_type(r->dtype, [&](auto dt) {
-      small_tile<decltype(dt)::value>(r->V, [&](auto t) { n = dmv_ceil_div(r->rows, kSmallThreads / decltype(t)::L); });
+      small_tile<decltype(dt)::value>(r->V, [&](auto t) { n = decltype(t)::groups(r->rows); });
     });
   return n;
 }
@@ -1747,7 +1876,7 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
     by_type(r->dtype, [&](auto dt) {
       small_tile<decltype(dt)::value>(r->V, [&](auto tile) {
         typedef decltype(tile) T;
-        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)n_loss, kSmallThreads, 0, st>>>(a);
+        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)n_loss, kSmallThreads, small_lds<T>(t->k), st>>>(a);
       });
     });
   } else if (row_fits(r->rows, r->V, r->dtype)) {
@@ -1794,8 +1923,7 @@ extern "C" int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher
     if (r->V <= kSmallMax) {
       small_tile<DT>(r->V, [&](auto tile) {
         typedef decltype(tile) T;
-        const int64_t groups = (r->rows + kSmallThreads / T::L - 1) / (kSmallThreads / T::L);
-        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)groups, kSmallThreads, 0, st>>>(a);
+        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)T::groups(r->rows), kSmallThreads, small_lds<T>(t->k), st>>>(a);
       });
     } else {
       a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);

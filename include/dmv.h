@@ -524,7 +524,7 @@ int dmv_grid_divergences(int32_t gen_dist, int32_t D, int32_t Zd, int64_t Nz, co
 enum { DMV_F32 = 0, DMV_BF16 = 1, DMV_F16 = 2 };
 #define DMV_CAT_MAX_TOP 64
 #define DMV_CAT_MAX_TEACHER 256
-#define DMV_CAT_SHORT_ROW 1024
+#define DMV_CAT_SHORT_ROW 2048
 typedef struct DmvCatRows {
   const void* logits;
   int64_t ld;

@@ -114,7 +114,7 @@ def test_log_prob_entry_refuses(args, code):
 def test_log_prob_entry_needs_x_and_workspace():
     lib = L.lib()
     assert lib.dmv_cat_log_prob(C.byref(_rows(X=None)), FAKE, None, 0, None, None, None, None, 0, None) == BAD
-    r = _rows(V=50000, ld=50000)
+    r = _rows(V=1 << 20, ld=1 << 20)
     need = lib.dmv_cat_log_prob_ws_bytes(C.byref(r), 5)
     assert need > 0 and need % 8 == 0
     for ws, n in ((None, 0), (FAKE, need - 1)):
