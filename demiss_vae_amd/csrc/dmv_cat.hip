@@ -132,16 +132,6 @@ __device__ __forceinline__ float log1p_row(float r) {
 
 __device__ __forceinline__ float exp2_hw(float d) { return __builtin_amdgcn_exp2f(d); }
 
-template <int R>
-__device__ __forceinline__ float gmax(float v) {
-  if (R >= 2) v = fmaxf(v, dpp_move<0xB1>(v));
-  if (R >= 4) v = fmaxf(v, dpp_move<0x4E>(v));
-  if (R >= 8) v = fmaxf(v, dpp_move<0x141>(v));
-  if (R >= 16) v = fmaxf(v, dpp_move<0x140>(v));
-  if (R >= 32) v = fmaxf(v, __shfl_xor(v, 16));
-  if (R >= 64) v = fmaxf(v, __shfl_xor(v, 32));
-  return v;
-}
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_move_u(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
@@ -155,6 +145,21 @@ __device__ __forceinline__ uint32_t gmax_u(uint32_t v) {
   if (R >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
   if (R >= 64) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
   return v;
+}
+
+// Largest of R lanes' values, as integers of the same order: a float maximum costs two more instructions a step (its
+// operands' NaNs are quietened first), an integer one takes the lane exchange as an operand.
+template <int R>
+__device__ __forceinline__ float gmax(float v) {
+  const int b = __float_as_int(v);
+  int k = b ^ ((b >> 31) & 0x7fffffff);
+  if (R >= 2) k = max(k, (int)dpp_move_u<0xB1>((uint32_t)k));
+  if (R >= 4) k = max(k, (int)dpp_move_u<0x4E>((uint32_t)k));
+  if (R >= 8) k = max(k, (int)dpp_move_u<0x141>((uint32_t)k));
+  if (R >= 16) k = max(k, (int)dpp_move_u<0x140>((uint32_t)k));
+  if (R >= 32) k = max(k, __shfl_xor(k, 16));
+  if (R >= 64) k = max(k, __shfl_xor(k, 32));
+  return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
 }
 
 // ------------------------------------------------------------------------------------------ arguments
@@ -348,46 +353,29 @@ template <bool ENT, int L, int E>
 __device__ __forceinline__ void small_stats(const float* o, float c, float& m, float& r, float& u) {
   m = gmax<L>(max_of<E>(o, -INFINITY));
   const float ref = m == -INFINITY ? 0.f : m;
-  // in blocks of eight: left alone, the scheduler holds every element's difference and exponential at once
-  float s = 0.f, t = 0.f;
+  // The largest element's term is 1 and all others' are below (or round to 1, and count as such): the fractions sum to
+  // those of the others, and what the whole sum has more is the number of ones.  (In blocks of eight: left alone, the
+  // scheduler holds every element's difference and exponential at once.)
+  float s = 0.f, f = 0.f, t = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (e % 8 == 0) __builtin_amdgcn_sched_barrier(0);
     const float d = (o[e] - ref) * c, w = exp2_hw(d);
     s += w;
+    f += __builtin_amdgcn_fractf(w);
     if (ENT) t = fmaf(w, fmaxf(d, kClampD), t);
   }
   u = ENT ? -gsum<L>(t) : 0.f;
-  r = gsum<L>(s) - 1.f;
-  if (r < kNearCertain && r >= 0.f) {
-    s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (e % 8 == 0) __builtin_amdgcn_sched_barrier(0);
-      s += o[e] < m ? exp2_hw((o[e] - m) * c) : 0.f;
-    }
-    r = gsum<L>(s);
-  }
+  const float others = gsum<L>(f);
+  r = others + (rintf(gsum<L>(s) - others) - 1.f);
 }
 
 // The k largest of a row held by L lanes, through emit(rank, value, index) by any lane; index -1 past the finite values.
 //
-// Few of them (k <= L, 8 or more lanes): the lanes fall into at least k sets; the smallest of the sets' largest values is a
-// lower bound of the k-th largest value, which about k ln k elements reach.  Those go to the group's list in LDS and are
+// Few of them (k <= L, 8 or more lanes): the k-th largest of the 2 L largest values of half a lane's elements is a lower
+// bound of the k-th largest element, which little more than k elements reach.  Those go to the group's list in LDS and are
 // ranked by counting.  Otherwise, or when the list is too short for them, one rank at a time.
 constexpr int kSmallList = 8;            // list entries per lane
-template <int L>
-__device__ __forceinline__ float sets_min(float mx, int k) {
-  // sets of L / S lanes, S >= k a power of two: the largest within, the smallest across
-  auto step = [&](float other, bool across) { mx = across ? fminf(mx, other) : fmaxf(mx, other); };
-  if (L >= 2) step(dpp_move<0xB1>(mx), k > L / 2);
-  if (L >= 4) step(dpp_move<0x4E>(mx), k > L / 4);
-  if (L >= 8) step(dpp_move<0x141>(mx), k > L / 8);
-  if (L >= 16) step(dpp_move<0x140>(mx), k > L / 16);
-  if (L >= 32) step(__shfl_xor(mx, 16), k > L / 32);
-  if (L >= 64) step(__shfl_xor(mx, 32), k > L / 64);
-  return mx;
-}
 // lanes of one wavefront that read what others of it wrote: in order without a wait
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -396,9 +384,20 @@ __device__ __forceinline__ void wave_sync() {
 template <int DT, int VEC, int L, int SL, typename Emit>
 __device__ __forceinline__ void small_top(const float* o, const char* p, int V, int lane, int k, cand_t* list, int* count, Emit emit) {
   constexpr int E = VEC * SL;
+  static_assert(E <= 32, "");
   auto index = [&](int j, int e) { return slot_base<VEC>(lane + L * j, V) + e; };
   if (L >= 8 && k <= L) {
-    const float bound = fmaxf(sets_min<L>(max_of<E>(o, -INFINITY), k), -3.402823466e38f);      // -inf is no alternative
+    float hi = max_of<E / 2>(o, -INFINITY), lo = max_of<E / 2>(o + E / 2, -INFINITY), bound;
+    const float both = fminf(hi, lo);
+    hi = fmaxf(hi, lo), lo = both;
+    for (int t = k;;) {
+      bound = gmax<L>(hi);
+      if (--t == 0) break;
+      const bool mine = hi == bound;
+      hi = mine ? lo : hi;
+      lo = mine ? -INFINITY : lo;
+    }
+    bound = fmaxf(bound, -3.402823466e38f);      // -inf is no alternative
     uint32_t bits = 0;
 #pragma unroll
     for (int i = E - 1; i >= 0; --i) bits = bits + bits + (o[i] >= bound ? 1u : 0u);
@@ -406,17 +405,21 @@ __device__ __forceinline__ void small_top(const float* o, const char* p, int V, 
     wave_sync();
     if (bits) {
       int at = atomicAdd(count, __popc(bits));
-      do {          // few: their values are read again rather than picked from registers
+      do {
         const int i = __ffs(bits) - 1;
         bits &= bits - 1;
-        const int at_v = index(i / VEC, i % VEC);
-        if (at < kSmallList * L) list[at] = candidate(order_key(Elem<DT>::load(p, at_v)), (uint32_t)at_v);
+        if (at < kSmallList * L) list[at] = (cand_t)(lane << 5 | i);
         ++at;
       } while (bits);
     }
     wave_sync();
     const int have = *count;
     if (have <= kSmallList * L) {
+      for (int q = lane; q < have; q += L) {      // (their values are read again rather than picked from registers)
+        const int id = (int)list[q], i = id & 31, at = slot_base<VEC>((id >> 5) + L * (i / VEC), V) + i % VEC;
+        list[q] = candidate(order_key(Elem<DT>::load(p, at)), (uint32_t)at);
+      }
+      wave_sync();
       for (int i = lane; i < have; i += L) {
         const cand_t me = list[i];
         int rank = 0;
