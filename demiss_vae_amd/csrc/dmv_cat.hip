@@ -372,32 +372,46 @@ __device__ __forceinline__ void small_stats(const float* o, float c, float& m, f
 
 // The k largest of a row held by L lanes, through emit(rank, value, index) by any lane; index -1 past the finite values.
 //
-// Few of them (k <= L, 8 or more lanes): the k-th largest of the 2 L largest values of half a lane's elements is a lower
-// bound of the k-th largest element, which little more than k elements reach.  Those go to the group's list in LDS and are
-// ranked by counting.  Otherwise, or when the list is too short for them, one rank at a time.
+// The k-th largest of the largest values of NB parts of every lane's elements, k <= L NB / 2, is a lower bound of the k-th
+// largest element, which little more than k elements reach.  Those go to the group's list in LDS and are ranked by
+// counting.  When the list is too short for them (many equal values): one rank at a time.
 constexpr int kSmallList = 8;            // list entries per lane
 // lanes of one wavefront that read what others of it wrote: in order without a wait
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+template <int NB, int E, int L>
+__device__ __forceinline__ float small_bound(const float* o, int k) {
+  constexpr int B = NB < E ? NB : E;          // (a tile of few elements has no more parts than those)
+  float mx[B];
+#pragma unroll
+  for (int b = 0; b < B; ++b) mx[b] = max_of<E / B>(o + b * (E / B), -INFINITY);
+#pragma unroll
+  for (int i = 1; i < B; ++i)                 // in order, largest first
+#pragma unroll
+    for (int j = i; j > 0; --j) {
+      const float hi = max3(mx[j - 1], mx[j], mx[j]), lo = fminf(mx[j - 1], mx[j]);
+      mx[j - 1] = hi, mx[j] = lo;
+    }
+  float bound;
+  for (int t = k;;) {
+    bound = gmax<L>(mx[0]);
+    if (--t == 0) break;
+    const bool mine = mx[0] == bound;
+#pragma unroll
+    for (int b = 0; b + 1 < B; ++b) mx[b] = mine ? mx[b + 1] : mx[b];
+    mx[B - 1] = mine ? -INFINITY : mx[B - 1];
+  }
+  return fmaxf(bound, -3.402823466e38f);      // -inf is no alternative
+}
 template <int DT, int VEC, int L, int SL, typename Emit>
 __device__ __forceinline__ void small_top(const float* o, const char* p, int V, int lane, int k, cand_t* list, int* count, Emit emit) {
   constexpr int E = VEC * SL;
   static_assert(E <= 32, "");
   auto index = [&](int j, int e) { return slot_base<VEC>(lane + L * j, V) + e; };
-  if (L >= 8 && k <= L) {
-    float hi = max_of<E / 2>(o, -INFINITY), lo = max_of<E / 2>(o + E / 2, -INFINITY), bound;
-    const float both = fminf(hi, lo);
-    hi = fmaxf(hi, lo), lo = both;
-    for (int t = k;;) {
-      bound = gmax<L>(hi);
-      if (--t == 0) break;
-      const bool mine = hi == bound;
-      hi = mine ? lo : hi;
-      lo = mine ? -INFINITY : lo;
-    }
-    bound = fmaxf(bound, -3.402823466e38f);      // -inf is no alternative
+  {
+    const float bound = k <= L ? small_bound<2, E, L>(o, k) : (k <= 2 * L ? small_bound<4, E, L>(o, k) : small_bound<8, E, L>(o, k));
     uint32_t bits = 0;
 #pragma unroll
     for (int i = E - 1; i >= 0; --i) bits = bits + bits + (o[i] >= bound ? 1u : 0u);
@@ -455,10 +469,97 @@ __device__ __forceinline__ void small_top(const float* o, const char* p, int V, 
   }
 }
 
-template <int DT, int VEC, int L, int SL, bool ENT, bool TOP>
+// All of a row's elements in order, for k beyond the bound's reach (k > 4 L): a bitonic network over the E L elements, pairs
+// within a lane or between lanes one or more apart.  Keys as candidate(); 16-bit types put their 16-bit key and the index
+// into 32 bits, which halves the exchanges (and a comparison costs two instructions instead of five).
+template <int DT>
+struct SortKey {
+  typedef uint32_t type;
+  static __device__ __forceinline__ type of(float x, int i) {
+    uint32_t k;
+    if constexpr (DT == DMV_BF16) {
+      k = order_key(x) >> 16;
+    } else {
+      const uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)(x + 0.f));
+      k = b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+    }
+    return x > -INFINITY ? k << 16 | (~(uint32_t)i & 0xffffu) : 0u;
+  }
+  static __device__ __forceinline__ int index(type k) { return (int)(~k & 0xffffu); }
+  static __device__ __forceinline__ float value(type k) {
+    const uint32_t h = k >> 16;
+    if constexpr (DT == DMV_BF16) return key_value(h & 0x8000u ? h << 16 : h << 16 | 0xffffu);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(h & 0x8000u ? h & 0x7fffu : ~h));
+  }
+};
+template <>
+struct SortKey<DMV_F32> {
+  typedef cand_t type;
+  static __device__ __forceinline__ type of(float x, int i) { return x > -INFINITY ? candidate(order_key(x), (uint32_t)i) : 0ull; }
+  static __device__ __forceinline__ int index(type k) { return (int)~(uint32_t)k; }
+  static __device__ __forceinline__ float value(type k) { return key_value((uint32_t)(k >> 32)); }
+};
+// the key of lane ^ X, X = 1, 2 or 4
+template <int X>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t k) {
+  if (X == 1) return dpp_move_u<0xB1>(k);
+  if (X == 2) return dpp_move_u<0x4E>(k);
+  return dpp_move_u<0x141>(dpp_move_u<0x1B>(k));        // 7 - (3 - lane within a quad): lane ^ 4
+}
+template <int X>
+__device__ __forceinline__ cand_t lane_xor(cand_t k) {
+  return (cand_t)lane_xor<X>((uint32_t)(k >> 32)) << 32 | lane_xor<X>((uint32_t)k);
+}
+template <int E, int SIZE, int STRIDE, typename K>
+__device__ __forceinline__ void sort_stage(K* key, int lane) {
+  // element lane E + e, largest first: a pair (i, i ^ STRIDE) is in descending order where i & SIZE is 0
+  if constexpr (STRIDE >= E) {
+    const bool low = (lane & (STRIDE / E)) == 0, down = (lane * E & SIZE) == 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const K other = lane_xor<STRIDE / E>(key[e]);
+      key[e] = ((low == down) == (other > key[e])) ? other : key[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if ((e & STRIDE) == 0) {
+        const bool down = SIZE < E ? (e & SIZE) == 0 : (lane * E & SIZE) == 0;
+        const K a = key[e], b = key[e | STRIDE];
+        const bool swap = (b > a) == down;
+        key[e] = swap ? b : a;
+        key[e | STRIDE] = swap ? a : b;
+      }
+  }
+  if constexpr (STRIDE > 1) sort_stage<E, SIZE, STRIDE / 2>(key, lane);
+}
+template <int E, int L, int SIZE, typename K>
+__device__ __forceinline__ void sort_down(K* key, int lane) {
+  if constexpr (SIZE > 2) sort_down<E, L, SIZE / 2>(key, lane);
+  sort_stage<E, SIZE, SIZE / 2>(key, lane);
+}
+template <int DT, int VEC, int L, int SL, typename Emit>
+__device__ __forceinline__ void small_sorted(const float* o, int V, int lane, int k, Emit emit) {
+  constexpr int E = VEC * SL;
+  typename SortKey<DT>::type key[E];
+#pragma unroll
+  for (int j = 0; j < SL; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) key[j * VEC + e] = SortKey<DT>::of(o[j * VEC + e], slot_base<VEC>(lane + L * j, V) + e);
+  sort_down<E, L, E * L>(key, lane);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int rank = lane * E + e;
+    if (rank < k) emit(rank, SortKey<DT>::value(key[e]), key[e] ? SortKey<DT>::index(key[e]) : -1);
+  }
+  for (int j = E * L + lane; j < k; j += L) emit(j, -INFINITY, -1);
+}
+
+enum { kNoTop = 0, kRanked = 1, kSorted = 2 };
+template <int DT, int VEC, int L, int SL, bool ENT, int TOP>
 __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
   constexpr int E = VEC * SL, NG = kSmallThreads / L, ES = sizeof(typename Elem<DT>::type);
-  __shared__ cand_t lists[TOP && L >= 8 ? NG : 1][TOP && L >= 8 ? kSmallList * L : 1];
+  __shared__ cand_t lists[TOP == kRanked ? NG : 1][TOP == kRanked ? kSmallList * L : 1];
   __shared__ int counts[NG];
   const int lane = threadIdx.x & (L - 1), V = a.r.V;
   const int row = blockIdx.x * NG + threadIdx.x / L;          // (rows * 16 bytes fit 32 bits)
@@ -491,17 +592,19 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
     if (ENT) a.entropy[(uint32_t)row] = H;
     if (a.stats) a.stats[(uint32_t)row] = f32x4{m, inv_s, logs, H};
   }
-  if constexpr (TOP) {
+  if constexpr (TOP != kNoTop) {
     float* lp = a.top_lp + (int64_t)row * a.top;
     int64_t* idx = a.top_idx + (int64_t)row * a.top;
     if (logs != logs) {
       for (int j = lane; j < a.top; j += L) lp[j] = NAN, idx[j] = -1;
     } else {
-      const int g = threadIdx.x / L;
-      small_top<DT, VEC, L, SL>(o, p, V, lane, a.top, lists[TOP && L >= 8 ? g : 0], &counts[g], [&](int rank, float v, int i) {
+      auto emit = [&](int rank, float v, int i) {
         idx[rank] = i;
         lp[rank] = i < 0 ? -INFINITY : (v - m) - logs;
-      });
+      };
+      const int g = threadIdx.x / L;
+      if constexpr (TOP == kSorted) small_sorted<DT, VEC, L, SL>(o, V, lane, a.top, emit);
+      else small_top<DT, VEC, L, SL>(o, p, V, lane, a.top, lists[TOP == kRanked ? g : 0], &counts[g], emit);
     }
   }
 }
@@ -836,6 +939,7 @@ __device__ __forceinline__ void block_join(const Online& on, float c, JoinShared
 
 constexpr int kRowThreads = 256;
 constexpr int kWideThreads = 1024;      // few rows
+constexpr int64_t kSingleRows = 4096, kSingleSlots = 2048;     // many rows of moderate length: one wavefront each
 constexpr int kUnroll = 4;              // slots in flight per thread
 constexpr int kGroups = 8;              // slot groups whose maxima a thread keeps for the selection
 constexpr int kCand = 512;              // candidates of a selection
@@ -846,7 +950,7 @@ constexpr int kMaxima = 4;              // largest values a lane holds in the se
 template <int NT>
 struct TopShared {
   float gm[kGroups][NT];               // largest value of a thread's slot group
-  float tmax[NT];
+  float tmax[NT < 256 ? 256 : NT];
   uint16_t list[kGroups * NT];
   cand_t cand[kCand + kCandPad];
   int groups, count;
@@ -886,8 +990,7 @@ __device__ __forceinline__ uint32_t lower_bound_of(const uint32_t* g, uint32_t t
 template <int NT, typename Emit>
 __device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, Emit emit) {
   const int tid = threadIdx.x;
-  static_assert(NT >= kCandPad, "");
-  if (tid < kCandPad) cand[have + tid] = 0;
+  for (int i = tid; i < kCandPad; i += NT) cand[have + i] = 0;
   __syncthreads();
   int sh = 0;
   while (sh < 4 && (have << (sh + 1)) <= NT) ++sh;
@@ -924,7 +1027,15 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, int V, int n, int s0
   const int tid = threadIdx.x, lane = tid & 63;
   const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
   if (tid == 0) sh.count = sh.groups = 0;
-  sh.tmax[tid] = tmax;
+  if constexpr (NT == 64) {      // a wavefront by itself: four sets of its slot groups
+#pragma unroll
+    for (int w = 0; w < kMaxima; ++w) {
+      const float a = w < groups ? sh.gm[w][tid] : -INFINITY, b = w + kMaxima < groups ? sh.gm[w + kMaxima][tid] : -INFINITY;
+      sh.tmax[64 * w + lane] = fmaxf(a, b);
+    }
+  } else {
+    sh.tmax[tid] = tmax;
+  }
   __syncthreads();
   if (tid < 64) {          // one wavefront searches: the others would only contend with it
     uint32_t g[kMaxima];
@@ -1694,6 +1805,9 @@ void by_type(int dt, F f) {
 // Few rows: sixteen wavefronts to each, where four would have more than one round of loads.
 bool wide_rows(int64_t groups, int V, int dt) { return groups <= 256 && V > kRowThreads * kUnroll * vec_elems(dt); }
 
+// Many rows that are not very long: a wavefront to each.
+bool single_wave_rows(int64_t groups, int V, int dt) { return groups >= kSingleRows && V <= kSingleSlots * vec_elems(dt); }
+
 // Workgroups per long row: one as long as its sixteen wavefronts need few rounds of loads (a join is another launch),
 // beyond that enough to occupy the chip.
 int parts_of(int64_t rows, int V, int dt) {
@@ -1725,6 +1839,7 @@ void launch_fwd_rows_by(const Fwd& a, bool entropy, hipStream_t st) {
 template <int DT>
 void launch_fwd_rows(const Fwd& a, bool entropy, hipStream_t st) {
   if (wide_rows(a.r.rows * a.parts, a.r.V / a.parts, DT)) launch_fwd_rows_by<DT, kWideThreads>(a, entropy, st);
+  else if (single_wave_rows(a.r.rows * a.parts, a.r.V / a.parts, DT)) launch_fwd_rows_by<DT, 64>(a, entropy, st);
   else launch_fwd_rows_by<DT, kRowThreads>(a, entropy, st);
 }
 
@@ -1765,13 +1880,15 @@ extern "C" int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* ent
       small_tile<decltype(dt)::value>(r->V, [&](auto t) {
         typedef decltype(t) T;
         const dim3 grid((unsigned)T::groups(r->rows)), block(kSmallThreads);
-        if (a.top) {
-          if (entropy) k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, true, true><<<grid, block, 0, st>>>(a);
-          else k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, false, true><<<grid, block, 0, st>>>(a);
-        } else {
-          if (entropy) k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, true, false><<<grid, block, 0, st>>>(a);
-          else k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, false, false><<<grid, block, 0, st>>>(a);
-        }
+        auto launch = [&](auto top) {
+          constexpr int TOP = decltype(top)::value;
+          if (entropy) k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, true, TOP><<<grid, block, 0, st>>>(a);
+          else k_cat_fwd_small<T::DT, T::VEC, T::L, T::SL, false, TOP><<<grid, block, 0, st>>>(a);
+        };
+        constexpr int parts = T::VEC * T::SL < 8 ? T::VEC * T::SL : 8;      // of a lane's elements, for the bound
+        if (!a.top) launch(std::integral_constant<int, kNoTop>());
+        else if (2 * a.top <= T::L * parts) launch(std::integral_constant<int, kRanked>());
+        else if constexpr (T::L <= 8) launch(std::integral_constant<int, kSorted>());
       });
     });
     DMV_HIP_CHECK_LAUNCH();
