@@ -136,14 +136,49 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_move_u(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
+// v of the other 16 lanes of 32, or of the other 32 lanes: the exchange gives each lane both its own and the other's, in
+// either order, which is all that a commutative operation needs
+template <int X, typename Op>
+__device__ __forceinline__ uint32_t across(uint32_t v, Op op) {
+  if constexpr (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return op(r[0], r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op(r[0], r[1]);
+  }
+}
 template <int R>
 __device__ __forceinline__ uint32_t gmax_u(uint32_t v) {
+  auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
   if (R >= 2) v = max(v, dpp_move_u<0xB1>(v));
   if (R >= 4) v = max(v, dpp_move_u<0x4E>(v));
   if (R >= 8) v = max(v, dpp_move_u<0x141>(v));
   if (R >= 16) v = max(v, dpp_move_u<0x140>(v));
-  if (R >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
-  if (R >= 64) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
+  if (R >= 32) v = across<16>(v, larger);
+  if (R >= 64) v = across<32>(v, larger);
+  return v;
+}
+template <int R>
+__device__ __forceinline__ uint32_t rsum_u(uint32_t v) {
+  auto add = [](uint32_t a, uint32_t b) { return a + b; };
+  if (R >= 2) v += dpp_move_u<0xB1>(v);
+  if (R >= 4) v += dpp_move_u<0x4E>(v);
+  if (R >= 8) v += dpp_move_u<0x141>(v);
+  if (R >= 16) v += dpp_move_u<0x140>(v);
+  if (R >= 32) v = across<16>(v, add);
+  if (R >= 64) v = across<32>(v, add);
+  return v;
+}
+template <int R>
+__device__ __forceinline__ float rsum(float v) {
+  auto add = [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
+  if (R >= 2) v += dpp_move<0xB1>(v);
+  if (R >= 4) v += dpp_move<0x4E>(v);
+  if (R >= 8) v += dpp_move<0x141>(v);
+  if (R >= 16) v += dpp_move<0x140>(v);
+  if (R >= 32) v = __uint_as_float(across<16>(__float_as_uint(v), add));
+  if (R >= 64) v = __uint_as_float(across<32>(__float_as_uint(v), add));
   return v;
 }
 
@@ -157,8 +192,9 @@ __device__ __forceinline__ float gmax(float v) {
   if (R >= 4) k = max(k, (int)dpp_move_u<0x4E>((uint32_t)k));
   if (R >= 8) k = max(k, (int)dpp_move_u<0x141>((uint32_t)k));
   if (R >= 16) k = max(k, (int)dpp_move_u<0x140>((uint32_t)k));
-  if (R >= 32) k = max(k, __shfl_xor(k, 16));
-  if (R >= 64) k = max(k, __shfl_xor(k, 32));
+  auto larger = [](uint32_t a, uint32_t b) { return (uint32_t)max((int)a, (int)b); };
+  if (R >= 32) k = (int)across<16>((uint32_t)k, larger);
+  if (R >= 64) k = (int)across<32>((uint32_t)k, larger);
   return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
 }
 
@@ -365,9 +401,9 @@ __device__ __forceinline__ void small_stats(const float* o, float c, float& m, f
     f += __builtin_amdgcn_fractf(w);
     if (ENT) t = fmaf(w, fmaxf(d, kClampD), t);
   }
-  u = ENT ? -gsum<L>(t) : 0.f;
-  const float others = gsum<L>(f);
-  r = others + (rintf(gsum<L>(s) - others) - 1.f);
+  u = ENT ? -rsum<L>(t) : 0.f;
+  const float others = rsum<L>(f);
+  r = others + (rintf(rsum<L>(s) - others) - 1.f);
 }
 
 // The k largest of a row held by L lanes, through emit(rank, value, index) by any lane; index -1 past the finite values.
@@ -381,12 +417,38 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+constexpr int kPops = 16;               // up to here the bound is found by taking the largest value k times
 template <int NB, int E, int L>
 __device__ __forceinline__ float small_bound(const float* o, int k) {
   constexpr int B = NB < E ? NB : E;          // (a tile of few elements has no more parts than those)
   float mx[B];
 #pragma unroll
   for (int b = 0; b < B; ++b) mx[b] = max_of<E / B>(o + b * (E / B), -INFINITY);
+  if (k > kPops) {
+    // the bound's bits one by one, below the exponent of the largest value if k values share it, until not many more than
+    // k reach it
+    uint32_t key[B];
+    float first = mx[0];
+#pragma unroll
+    for (int b = 0; b < B; ++b) key[b] = order_key(mx[b]), first = fmaxf(first, mx[b]);
+    auto reach = [&](uint32_t t) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int b = 0; b < B; ++b) c += key[b] >= t ? 1u : 0u;
+      return (int)rsum_u<L>(c);
+    };
+    const uint32_t start = order_key(gmax<L>(first)) & 0xff800000u;
+    int c = reach(start);
+    const bool near = c >= k;
+    uint32_t tau = near ? start : 0u;
+    const int enough = k + (k >> 2) + 1;
+    for (int bit = near ? 22 : 31; bit >= 0 && !(tau != 0u && c <= enough); --bit) {
+      const uint32_t t = tau | (1u << bit);
+      const int ct = reach(t);
+      if (ct >= k) tau = t, c = ct;
+    }
+    return tau <= kKeyMinusInf ? -3.402823466e38f : fmaxf(key_value(tau), -3.402823466e38f);
+  }
 #pragma unroll
   for (int i = 1; i < B; ++i)                 // in order, largest first
 #pragma unroll
@@ -634,7 +696,7 @@ __device__ __forceinline__ RowGrad row_grad(const Bwd& a, int64_t row, int lane,
     float s = 0.f;
     for (int j = lane; j < a.top; j += R)
       if (a.top_idx[row * a.top + j] >= 0) s += a.g_top[row * a.top + j];
-    g.S += gsum<R>(s);
+    g.S += rsum<R>(s);
   }
   g.gh = a.g_ent ? a.g_ent[row] : 0.f;
   g.m = g.inv_s = g.logs = g.H = 0.f;
@@ -754,7 +816,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
           if (own[j].p == tm) held += 1.f;
           else s += exp2_hw((own[j].p - tm) * a.t.c);
         }
-      const float t_logs = log1p_row(gsum<L>(s) + (gsum<L>(held) - 1.f));
+      const float t_logs = log1p_row(rsum<L>(s) + (rsum<L>(held) - 1.f));
       for (int j = lane; j < K; j += L)
         if (own[j].i >= 0) {
           const float lp = (own[j].p - tm) * a.t.inv_T - t_logs, q = expf(lp), lq = (own[j].lq - m) * a.t.inv_T - logs;
@@ -762,7 +824,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
           own[j].p = q;
           own[j].lq = lq;
         }
-      kl = gsum<L>(kl);
+      kl = rsum<L>(kl);
     }
     if (any && empty) kl = INFINITY;
     if (bad) kl = NAN;
@@ -850,7 +912,7 @@ __device__ __forceinline__ float block_max(float v, BlockRed<NT>& s) {
 }
 template <int NT>
 __device__ __forceinline__ void block_sum3(float& p, float& q, float& w, BlockRed<NT>& s) {
-  p = gsum<64>(p), q = gsum<64>(q), w = gsum<64>(w);
+  p = rsum<64>(p), q = rsum<64>(q), w = rsum<64>(w);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
     s.x[0][threadIdx.x >> 6] = p;
@@ -898,9 +960,9 @@ __device__ __forceinline__ void join_sets(float& m, float& r, float& u, float c)
   const float top = gmax<R>(m), ref = top == -INFINITY ? 0.f : top;
   const float shift = fmaxf((m - ref) * c, kClampD), f = exp2_hw(shift);
   const bool holds = m == top && m != -INFINITY;
-  const float others = gsum<R>(holds ? r : f * (1.f + r));
-  u = gsum<R>(f * (u - (1.f + r) * shift));
-  r = others + (gsum<R>(holds ? 1.f : 0.f) - 1.f);
+  const float others = rsum<R>(holds ? r : f * (1.f + r));
+  u = rsum<R>(f * (u - (1.f + r) * shift));
+  r = others + (rsum<R>(holds ? 1.f : 0.f) - 1.f);
   m = top;
 }
 
@@ -919,7 +981,7 @@ __device__ __forceinline__ void block_join(const Online& on, float c, JoinShared
   const float shift = fmaxf((on.m - wref) * c, kClampD), f = exp2_hw(shift);
   const bool holds = on.m == wm;
   const unsigned long long who = __ballot(holds);
-  const float a = gsum<64>(holds ? on.s - 1.f : on.s * f), b = ENT ? -gsum<64>(f * fmaf(on.s, shift, on.t)) : 0.f;
+  const float a = rsum<64>(holds ? on.s - 1.f : on.s * f), b = ENT ? -rsum<64>(f * fmaf(on.s, shift, on.t)) : 0.f;
   if (lane == 0) sh.wave[wave] = f32x4{wm, wm == -INFINITY && a == a ? -1.f : a + ((float)__popcll(who) - 1.f), b,
                                        __int_as_float(wave * 64 + __ffsll(who) - 1)};
   __syncthreads();
@@ -930,10 +992,10 @@ __device__ __forceinline__ void block_join(const Online& on, float c, JoinShared
   else if (r < kNearCertain) {                     // one thread holds the largest: its sum has rounded the rest away
     const int w = __ffsll(__ballot(mine[0] == m)) - 1, holder = __float_as_int(__shfl(mine[3], w));
     const float mshift = fmaxf((on.m - m) * c, kClampD);
-    const float again = gsum<64>(resum(holder, m) + ((int)threadIdx.x == holder ? 0.f : on.s * exp2_hw(mshift)));
+    const float again = rsum<64>(resum(holder, m) + ((int)threadIdx.x == holder ? 0.f : on.s * exp2_hw(mshift)));
     if (lane == 0) sh.again[wave] = again;
     __syncthreads();
-    r = gsum<W>(sh.again[lane & (W - 1)]);
+    r = rsum<W>(sh.again[lane & (W - 1)]);
   }
 }
 
@@ -1221,11 +1283,12 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
   const int per = ((ns + a.parts - 1) / a.parts + 15) & ~15;      // equal to 16 slots
   const int s0 = part * per < ns ? part * per : ns, s1 = s0 + per < ns ? s0 + per : ns;
   const char* p = a.r.x + row * a.r.ld * ES;
-  int gsz = (s1 - s0 + NT * kGroups - 1) / (NT * kGroups);    // slots per group of the selection
-  gsz = gsz < kUnroll ? kUnroll : (gsz + kUnroll - 1) / kUnroll * kUnroll;
+  int gsz = (s1 - s0 + NT * kGroups - 1) / (NT * kGroups);    // slots per group of the selection: 1, 2 or whole rounds
+  gsz = gsz <= 2 ? (gsz < 1 ? 1 : gsz) : (gsz + kUnroll - 1) / kUnroll * kUnroll;
   Online on;
   float gmx = -INFINITY;
   int in_group = 0, group = 0;
+  const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
   // IN slots in flight per thread, kUnroll at a time through the sums
   constexpr int IN = NT == kWideThreads ? 2 * kUnroll : kUnroll;
   for (int sb = s0 + tid; sb < s1; sb += NT * IN) {
@@ -1250,23 +1313,44 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
             if (sq >= s1 || b + e < sq * VEC || b + e >= n) v[q * VEC + e] = -INFINITY;
         }
       }
-      const float mx = max_of<kUnroll * VEC>(v, -INFINITY);
+      float mx;
       if constexpr (TOP) {
-        if (s < s1) {
-          gmx = max3(mx, gmx, gmx);
-          in_group += kUnroll;
-          if (in_group == gsz) {
-            top_sh.gm[group++][tid] = gmx;
-            gmx = -INFINITY;
-            in_group = 0;
+        float part[kUnroll];
+#pragma unroll
+        for (int q = 0; q < kUnroll; ++q) part[q] = max_of<VEC>(v + q * VEC, -INFINITY);
+        const float half0 = max3(part[0], part[1], part[1]), half1 = max3(part[2], part[3], part[3]);
+        mx = max3(half0, half1, half1);
+        static_assert(kUnroll == 4, "");
+        if (gsz >= kUnroll) {
+          if (s < s1) {
+            gmx = max3(mx, gmx, gmx);
+            in_group += kUnroll;
+            if (in_group == gsz) {
+              top_sh.gm[group++][tid] = gmx;
+              gmx = -INFINITY;
+              in_group = 0;
+            }
+          }
+        } else {
+          const int left = groups - group;       // (groups past the last one have no slots)
+          if (gsz == 1) {
+#pragma unroll
+            for (int q = 0; q < kUnroll; ++q)
+              if (q < left) top_sh.gm[group + q][tid] = part[q];
+            group += kUnroll;
+          } else {
+            if (0 < left) top_sh.gm[group][tid] = half0;
+            if (1 < left) top_sh.gm[group + 1][tid] = half1;
+            group += 2;
           }
         }
+      } else {
+        mx = max_of<kUnroll * VEC>(v, -INFINITY);
       }
       on.template add<kUnroll * VEC, ENT>(v, mx, a.c);
     }
   }
   if constexpr (TOP) {
-    const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
     for (; group < groups; ++group) {
       top_sh.gm[group][tid] = gmx;
       gmx = -INFINITY;
