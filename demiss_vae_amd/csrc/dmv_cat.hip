@@ -262,6 +262,7 @@ struct Dist {
   Teacher t;
   float* per_row;
   double* loss_part;  // one per workgroup of the launch
+  float* loss;        // the loss itself, if the launch has one workgroup
   f32x4* stats;
   const float* gscale;
   int unless_one;  // the gradient of gscale = 1 is already in place
@@ -334,20 +335,40 @@ constexpr int kSmallMax = DMV_CAT_SHORT_ROW;   // their longest row: 64 lanes, 3
 typedef unsigned long long cand_t;
 __device__ __forceinline__ cand_t candidate(uint32_t key, uint32_t index) { return ((cand_t)key << 32) | (uint32_t)~index; }
 
+// The values of a packed slot for one pass over the row.  The compiler is made to forget what it knows of them and to keep
+// the slots in order: it would otherwise hold the unpacked values, twice the registers, across the passes.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int DT>
+__device__ __forceinline__ void pass_over(u32x4& r, float* v) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" : "+v"(r));
+  Elem<DT>::unpack(__builtin_bit_cast(Raw16, r), v);
+}
+__device__ __forceinline__ int again(int t) {
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 template <int DT, int VEC>
 struct SmallSlot {
-  Raw16 raw;
+  u32x4 raw;
   __device__ __forceinline__ void load(const char* p, int base) {
-    raw = *(const Raw16*)(p + (int64_t)base * (int)sizeof(typename Elem<DT>::type));
+    raw = __builtin_bit_cast(u32x4, *(const Raw16*)(p + (int64_t)base * (int)sizeof(typename Elem<DT>::type)));
   }
-  __device__ __forceinline__ void unpack(float* v) const { Elem<DT>::unpack(raw, v); }
-  __device__ __forceinline__ void pack(const float* v) { Elem<DT>::pack(v, raw); }
+  __device__ __forceinline__ void unpack(float* v) const { Elem<DT>::unpack(__builtin_bit_cast(Raw16, raw), v); }
+  __device__ __forceinline__ void pass(float* v) { pass_over<DT>(raw, v); }
+  __device__ __forceinline__ void pack(const float* v) {
+    Raw16 r;
+    Elem<DT>::pack(v, r);
+    raw = __builtin_bit_cast(u32x4, r);
+  }
 };
 template <int DT>
 struct SmallSlot<DT, 1> {
   float x;
   __device__ __forceinline__ void load(const char* p, int base) { x = Elem<DT>::load(p, base); }
   __device__ __forceinline__ void unpack(float* v) const { v[0] = x; }
+  __device__ __forceinline__ void pass(float* v) { v[0] = x; }
   __device__ __forceinline__ void pack(const float* v) { x = v[0]; }
 };
 
@@ -384,22 +405,35 @@ struct SmallRow {
   }
 };
 
-// (m, r, u) of a row held by L lanes; r < 0: no category of non-zero probability
-template <bool ENT, int L, int E>
-__device__ __forceinline__ void small_stats(const float* o, float c, float& m, float& r, float& u) {
-  m = gmax<L>(max_of<E>(o, -INFINITY));
+// (m, r, u) of a row held by L lanes; r < 0: no category of non-zero probability.  The largest element's term is 1 and all
+// others' are below (or round to 1, and count as such): the fractions sum to those of the others, and what the whole sum
+// has more is the number of ones.  The row stays packed between the passes: unpacked it would take twice the registers,
+// and the kernel half of its wavefronts.
+// KEEP: the terms 2^(c (x - m)) go to `kept`.
+template <bool ENT, bool KEEP, int DT, int VEC, int L, int SL>
+__device__ __forceinline__ void small_stats(SmallRow<DT, VEC, L, SL>& x, float c, float& m, float& r, float& u, float* kept = nullptr) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    float v[VEC];
+    x.slot[j].pass(v);
+    mx = max_of<VEC>(v, mx);
+  }
+  m = gmax<L>(mx);
   const float ref = m == -INFINITY ? 0.f : m;
-  // The largest element's term is 1 and all others' are below (or round to 1, and count as such): the fractions sum to
-  // those of the others, and what the whole sum has more is the number of ones.  (In blocks of eight: left alone, the
-  // scheduler holds every element's difference and exponential at once.)
   float s = 0.f, f = 0.f, t = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (e % 8 == 0) __builtin_amdgcn_sched_barrier(0);
-    const float d = (o[e] - ref) * c, w = exp2_hw(d);
-    s += w;
-    f += __builtin_amdgcn_fractf(w);
-    if (ENT) t = fmaf(w, fmaxf(d, kClampD), t);
+  for (int j = 0; j < SL; ++j) {
+    float v[VEC];
+    x.slot[j].pass(v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = (v[e] - ref) * c, w = exp2_hw(d);
+      s += w;
+      f += __builtin_amdgcn_fractf(w);
+      if (ENT) t = fmaf(w, fmaxf(d, kClampD), t);
+      if (KEEP) kept[j * VEC + e] = w;
+    }
   }
   u = ENT ? -rsum<L>(t) : 0.f;
   const float others = rsum<L>(f);
@@ -642,10 +676,9 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
     given = X >= 0 && X < n;
     if (given) xX = Elem<DT>::load(p, X);
   }
-  float o[E], m, r, u;
+  float m, r, u;
   x.count_once(V, n, lane);
-  x.values(o);
-  small_stats<ENT, L, E>(o, a.c, m, r, u);
+  small_stats<ENT, false>(x, a.c, m, r, u);
   const bool empty = m == -INFINITY && !(r != r);
   const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
   const float H = empty ? 0.f : fmaf(kLn2 * u, inv_s, logs);
@@ -665,6 +698,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
         lp[rank] = i < 0 ? -INFINITY : (v - m) - logs;
       };
       const int g = threadIdx.x / L;
+      float o[E];
+      x.values(o);
       if constexpr (TOP == kSorted) small_sorted<DT, VEC, L, SL>(o, V, lane, a.top, emit);
       else small_top<DT, VEC, L, SL>(o, p, V, lane, a.top, lists[TOP == kRanked ? g : 0], &counts[g], emit);
     }
@@ -755,32 +790,42 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_bwd_small(Bwd a) {
 // themselves.  An index past the row's categories, or a logit that is NaN or +inf, makes the row's loss and gradient NaN.
 __device__ __forceinline__ bool entry_counts(float t, int64_t i) { return i >= 0 && t != -INFINITY; }
 
-// q - p without its cancellation
-__device__ __forceinline__ float q_minus_p(float lq, float p) {
-  const float q = expf(lq);
-  if (p > 0.5f * q) return p * expm1f(lq - logf(p));
-  return q - p;
+__device__ __forceinline__ float exp_hw(float x) { return exp2_hw(x * kLog2e); }
+// q - p of their logarithms without its cancellation: p expm1(log q - log p), a series where that is small
+__device__ __forceinline__ float q_minus_p(float lq, float lp) {
+  const float x = lq - lp, p = exp_hw(lp);
+  if (fabsf(x) < 0.35f)      // (the next term is below 2e-8 of the sum)
+    return p * (x * (1.f + x * (1.f / 2 + x * (1.f / 6 + x * (1.f / 24 + x * (1.f / 120 + x * (1.f / 720 + x * (1.f / 5040))))))));
+  return x < 1.f ? p * (exp_hw(x) - 1.f) : exp_hw(lq) - p;
 }
 
-// A teacher's entry in LDS: probability, log q of its category, category (-1: empty).
+// A teacher's entry in LDS: its logit, then log p; the student's logit, then log q of its category; category (-1: empty).
 struct Entry {
-  float p, lq;
+  float t, x;
   int i;
 };
 constexpr int kFewEntries = 16;       // up to here a category given twice is looked for entry by entry
+constexpr int kLoneThreads = 1024;    // the workgroup of a small launch, which also forms the loss: a second launch saved
 
-template <int DT, int VEC, int L, int SL>
-__global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
-  constexpr int E = VEC * SL, NG = kSmallThreads / L, ES = sizeof(typename Elem<DT>::type), WORDS = E * L / 32;
-  __shared__ double sums[kSmallThreads / 64];
+template <int DT, int VEC, int L>
+__device__ __forceinline__ void small_zeros(char* out, int V, int lane) {
+  const float z[VEC] = {};
+  for (int s = lane; s * VEC < V; s += L) slot_store<DT, VEC>(out, slot_base<VEC>(s, V), z);
+}
+
+template <int DT, int VEC, int L, int SL, int NT>
+__global__ void __launch_bounds__(NT) k_cat_distill_small(Dist a) {
+  constexpr int E = VEC * SL, ES = sizeof(typename Elem<DT>::type), WORDS = E * L / 32, NG = NT / L;
+  constexpr bool LONE = NT == kLoneThreads;
+  __shared__ double sums[NT / 64];
   __shared__ uint32_t given[NG][WORDS];
   extern __shared__ Entry entries[];    // [NG][k]
   const float gs = a.gscale ? *a.gscale : 1.f;
   if (a.unless_one && gs == 1.f) return;
   const int lane = threadIdx.x & (L - 1), V = a.r.V, K = a.t.k, g = threadIdx.x / L;
-  const int row = blockIdx.x * NG + g;
   double part = 0.0;
-  const float w = row >= (int)a.r.rows ? 0.f : (a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f);
+  for (int row = blockIdx.x * NG + g; row < (int)a.r.rows; row += NG) {
+  const float w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
   float kl = 0.f;
   if (w != 0.f) {
     const char* p = a.r.x + row * a.r.ld * ES;
@@ -802,10 +847,9 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
     tm = gmax<L>(tm);
     flags = gmax_u<L>(flags);
     const bool any = flags != 0u, bad = flags >= 2u;
-    float o[E], m, r, u;
+    float m, r, u, kept[E];
     x.count_once(V, n, lane);
-    x.values(o);
-    small_stats<false, L, E>(o, a.t.c, m, r, u);
+    small_stats<false, true>(x, a.t.c, m, r, u, kept);      // (twice the registers of the packed row, but no second exp2)
     const bool empty = m == -INFINITY && !(r != r);
     const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
     const bool live = any && !empty;
@@ -813,34 +857,33 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
       float s = 0.f, held = 0.f;
       for (int j = lane; j < K; j += L)
         if (own[j].i >= 0) {
-          if (own[j].p == tm) held += 1.f;
-          else s += exp2_hw((own[j].p - tm) * a.t.c);
+          if (own[j].t == tm) held += 1.f;
+          else s += exp2_hw((own[j].t - tm) * a.t.c);
         }
       const float t_logs = log1p_row(rsum<L>(s) + (rsum<L>(held) - 1.f));
       for (int j = lane; j < K; j += L)
         if (own[j].i >= 0) {
-          const float lp = (own[j].p - tm) * a.t.inv_T - t_logs, q = expf(lp), lq = (own[j].lq - m) * a.t.inv_T - logs;
+          const float lp = (own[j].t - tm) * a.t.inv_T - t_logs, q = exp_hw(lp), lq = (own[j].x - m) * a.t.inv_T - logs;
           if (q > 0.f) kl += q * (lp - lq);
-          own[j].p = q;
-          own[j].lq = lq;
+          own[j].t = lp;
+          own[j].x = lq;
         }
       kl = rsum<L>(kl);
     }
     if (any && empty) kl = INFINITY;
     if (bad) kl = NAN;
-    if (lane == 0) part = (double)w * (double)kl;
+    if (lane == 0) part += (double)w * (double)kl;
     if (a.d) {
       char* out = (char*)a.d + row * a.ld_d * ES;
-      const float scale = bad ? NAN : gs * w * a.t.inv_T, f = live ? scale * inv_s : 0.f;
+      const float scale = bad ? NAN : gs * w * a.t.inv_T, f = scale * inv_s;
+      if (!live) small_zeros<DT, VEC, L>(out, V, lane);
 #pragma unroll
       for (int j = 0; j < SL; ++j) {
         const int fst = (lane + L * j) * VEC;
-        if (fst >= V) continue;
-        __builtin_amdgcn_sched_barrier(0);
+        if (fst >= V || !live) continue;
         float v[VEC];
-        x.slot[j].unpack(v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = live ? f * exp2_hw((v[e] - m) * a.t.c) : 0.f;     // (what does not count: 0)
+        for (int e = 0; e < VEC; ++e) v[e] = f * kept[j * VEC + e];     // (what does not count: 0)
         if (fst + VEC <= V) slot_store<DT, VEC>(out, fst, v);
         else {
 #pragma unroll
@@ -867,30 +910,34 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_distill_small(Dist a) {
         for (int j = lane; j < K; j += L) {
           const Entry e = own[j];
           if (e.i < 0) continue;
-          float sum = e.p;
+          float lp = e.t;
           if (twice) {
-            sum = 0.f;
-            for (int h = 0; h < K; ++h) sum += own[h].i == e.i ? own[h].p : 0.f;
+            int same = 0;
+            float sum = 0.f;
+            for (int h = 0; h < K; ++h)
+              if (own[h].i == e.i) sum += exp_hw(own[h].t), ++same;
+            if (same > 1) lp = logf(sum);
           }
-          Elem<DT>::store(out, e.i, scale * q_minus_p(e.lq, sum));
+          Elem<DT>::store(out, e.i, scale * q_minus_p(e.x, lp));
         }
       }
     }
-  } else if (a.d && row < (int)a.r.rows) {
-    char* out = (char*)a.d + row * a.ld_d * ES;
-    const float z[VEC] = {};
-    for (int sl = lane; sl * VEC < V; sl += L) slot_store<DT, VEC>(out, slot_base<VEC>(sl, V), z);
+  } else if (a.d) {
+    small_zeros<DT, VEC, L>((char*)a.d + row * a.ld_d * ES, V, lane);
   }
-  if (lane == 0 && a.per_row && row < (int)a.r.rows) a.per_row[(uint32_t)row] = kl;
+  if (lane == 0 && a.per_row) a.per_row[(uint32_t)row] = kl;
+  if (!LONE) break;
+  }
   // the workgroup's share of the loss, in a fixed order
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) part += __shfl_xor(part, off);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = part;
   __syncthreads();
-  if (threadIdx.x == 0 && a.loss_part) {
+  if (threadIdx.x == 0 && (LONE ? a.loss != nullptr : a.loss_part != nullptr)) {
     double s = 0.0;
-    for (int i = 0; i < kSmallThreads / 64; ++i) s += sums[i];
-    a.loss_part[blockIdx.x] = s;
+    for (int i = 0; i < NT / 64; ++i) s += sums[i];
+    if (LONE) *a.loss = (float)s;
+    else a.loss_part[blockIdx.x] = s;
   }
 }
 
@@ -1578,7 +1625,7 @@ __device__ __forceinline__ TeacherEntry teacher_row(const Teacher& t, int64_t ro
   e.any = held > 0.f || e.bad;
   if (counts) {
     e.lp = (x - tm) * t.inv_T - log1p_row(s + (held - 1.f));
-    e.p = expf(e.lp);
+    e.p = exp_hw(e.lp);
   }
   return e;
 }
@@ -1587,25 +1634,14 @@ struct SparseShared {
   float p[kMaxTeacher];
   int i[kMaxTeacher];
 };
-// all of the teacher's probability on category i (it may be given more than once): the same sum for each of its entries
-__device__ __forceinline__ float share_of(const SparseShared& sh, int k, int i) {
+// log of all of the teacher's probability on entry e's category, which may be given more than once: the same for each of
+// its entries
+__device__ __forceinline__ float share_of(const SparseShared& sh, int k, const TeacherEntry& e) {
   float p = 0.f;
-  for (int j = 0; j < k; ++j) p += sh.i[j] == i ? sh.p[j] : 0.f;
-  return p;
-}
-
-// The values of a packed slot for one pass over the row.  The compiler is made to forget what it knows of them and to keep
-// the slots in order: it would otherwise hold the unpacked values, twice the registers, across the passes.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-template <int DT>
-__device__ __forceinline__ void pass_over(u32x4& r, float* v) {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" : "+v"(r));
-  Elem<DT>::unpack(__builtin_bit_cast(Raw16, r), v);
-}
-__device__ __forceinline__ int again(int t) {
-  asm volatile("" : "+v"(t));
-  return t;
+  int same = 0;
+  for (int j = 0; j < k; ++j)
+    if (sh.i[j] == e.i) p += sh.p[j], ++same;
+  return same > 1 ? logf(p) : e.lp;
 }
 
 // Loss and gradient of a row that fits the registers of one workgroup (NV slots per thread): the row is read once.
@@ -1723,7 +1759,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
     else chunk_store<DT>(out, s, V - VEC, v);
   }
   __syncthreads();          // the dense part before the teacher's categories are written again
-  if (te.i >= 0 && !te.bad) Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te.i)));
+  if (te.i >= 0 && !te.bad) Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te)));
 }
 
 // Rows that are read by several workgroups: their parts' statistics (k_cat_fwd_row) joined, and the loss.
@@ -1812,7 +1848,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_distill_chunk(Dist a) {
     const int64_t lo = (int64_t)s0 * VEC;
     if (live && !te.bad && te.i >= lo && te.i < lo + (int64_t)kChunkSlots * VEC) {
       const float lq = (Elem<DT>::load(p, te.i) - st[0]) * a.t.inv_T - st[2];
-      Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te.i)));
+      Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te)));
     }
     __syncthreads();        // sp is free again
   }
@@ -1934,8 +1970,8 @@ void launch_distill_row(const Dist& a, hipStream_t st) {
   if (ns <= 2 * 256) k_cat_distill_row<DT, 256, 2><<<grid, 256, 0, st>>>(a);
   else if (ns <= 4 * 256) k_cat_distill_row<DT, 256, 4><<<grid, 256, 0, st>>>(a);
   else if (ns <= 8 * 256) k_cat_distill_row<DT, 256, 8><<<grid, 256, 0, st>>>(a);
-  else if (ns <= 8 * 512) k_cat_distill_row<DT, 512, 8><<<grid, 512, 0, st>>>(a);
-  else if (ns <= 8 * 1024) k_cat_distill_row<DT, 1024, 8><<<grid, 1024, 0, st>>>(a);
+  else if (ns <= 16 * 256) k_cat_distill_row<DT, 256, 16><<<grid, 256, 0, st>>>(a);
+  else if (ns <= 16 * 512) k_cat_distill_row<DT, 512, 16><<<grid, 512, 0, st>>>(a);
   else k_cat_distill_row<DT, 1024, 16><<<grid, 1024, 0, st>>>(a);
 }
 
@@ -2037,6 +2073,11 @@ static Dist dist_of(const DmvCatRows* r, const DmvCatTeacher* t) {
   a.chunks = a.parts = 1;
   return a;
 }
+// A small launch: one workgroup does all rows in a few rounds, and the loss.
+template <typename T>
+bool lone_group(int64_t rows, int k) {
+  return rows <= 4 * (kLoneThreads / T::L) && (size_t)(kLoneThreads / T::L) * k * sizeof(Entry) <= 48 * 1024;
+}
 static int64_t loss_parts(const DmvCatRows* r) {
   int64_t n = r->rows;
   if (r->V <= kSmallMax)
@@ -2080,7 +2121,12 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
     by_type(r->dtype, [&](auto dt) {
       small_tile<decltype(dt)::value>(r->V, [&](auto tile) {
         typedef decltype(tile) T;
-        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)n_loss, kSmallThreads, small_lds<T>(t->k), st>>>(a);
+        if (lone_group<T>(r->rows, t->k)) {
+          a.loss = loss;
+          k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kLoneThreads><<<1, kLoneThreads, small_lds<T>(t->k) * (kLoneThreads / kSmallThreads), st>>>(a);
+        } else {
+          k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kSmallThreads><<<(unsigned)n_loss, kSmallThreads, small_lds<T>(t->k), st>>>(a);
+        }
       });
     });
   } else if (row_fits(r->rows, r->V, r->dtype)) {
@@ -2100,7 +2146,7 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
       if (a.d) k_cat_distill_chunk<DT><<<(unsigned)(items < 8192 ? items : 8192), kRowThreads, 0, st>>>(a);
     });
   }
-  k_cat_loss<<<1, kLossThreads, 0, st>>>(a.loss_part, n_loss, loss);
+  if (!a.loss) k_cat_loss<<<1, kLossThreads, 0, st>>>(a.loss_part, n_loss, loss);
   DMV_HIP_CHECK_LAUNCH();
   return DMV_OK;
 }
@@ -2127,7 +2173,7 @@ extern "C" int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher
     if (r->V <= kSmallMax) {
       small_tile<DT>(r->V, [&](auto tile) {
         typedef decltype(tile) T;
-        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL><<<(unsigned)T::groups(r->rows), kSmallThreads, small_lds<T>(t->k), st>>>(a);
+        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kSmallThreads><<<(unsigned)T::groups(r->rows), kSmallThreads, small_lds<T>(t->k), st>>>(a);
       });
     } else {
       a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
