@@ -285,6 +285,26 @@ __device__ __forceinline__ int slot_base(int s, int V) {
   const int b = s * VEC;
   return b + VEC <= V ? b : V - VEC;
 }
+// Slots of a long row, cut where its addresses are multiples of 16: slot s = elements [s VEC - lead, s VEC - lead + VEC) below
+// n.  Accesses stay inside the row as above; a first and a last slot overlap their neighbours.  (Cut at the row's start,
+// rows of odd length take a fifth longer to read: 1024 x 50001 float16 27 us, x 50000 23 us.)
+template <int VEC>
+struct Span {
+  int lead, V, n, slots;
+  __device__ __forceinline__ Span(const char* p, int elem, int V_, int n_) : V(V_), n(n_) {
+    lead = (int)(((uintptr_t)p & 15) / elem);
+    slots = n > 0 ? (n + lead + VEC - 1) / VEC : 0;
+  }
+  __device__ __forceinline__ int base(int s) const {
+    const int f = s * VEC - lead;
+    return f < 0 ? 0 : (f + VEC <= V ? f : V - VEC);
+  }
+  __device__ __forceinline__ bool whole(int s) const { return s * VEC >= lead && s * VEC - lead + VEC <= n; }
+  __device__ __forceinline__ bool holds(int s, int i) const {
+    const int f = s * VEC - lead;
+    return i >= f && i < f + VEC && i < n;
+  }
+};
 template <int DT, int VEC>
 __device__ __forceinline__ void slot_load(const char* row, int base, float* v) {
   if constexpr (VEC == 1) {
@@ -1131,7 +1151,7 @@ __device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, E
 // in an ordinary row - are ranked by counting.  Rows with more candidates than fit (many equal values) take the
 // ordered scan below, and in the worst case one pass over the listed groups per rank.
 template <int DT, int VEC, int NT, typename Emit>
-__device__ void block_top(TopShared<NT>& sh, const char* p, int V, int n, int s0, int s1, int gsz, int k, float m, float tmax,
+__device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& span, int s0, int s1, int gsz, int k, float m, float tmax,
                           Emit emit) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int groups = (s1 - s0 + NT * gsz - 1) / (NT * gsz);
@@ -1180,13 +1200,13 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, int V, int n, int s0
       const int s = s0 + (at & (NT - 1)) + NT * (at / NT * gsz + (j - l * gsz));
       if (s >= s1) continue;
       float v[VEC];
-      const int b = slot_base<VEC>(s, V);
+      const int b = span.base(s);
       slot_load<DT, VEC>(p, b, v);
       uint32_t key[VEC], bits = 0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         key[e] = order_key(v[e]);
-        if (b + e >= s * VEC && b + e < n && key[e] >= lowest) bits |= 1u << e;
+        if (span.holds(s, b + e) && key[e] >= lowest) bits |= 1u << e;
       }
       if (bits) f(key, b, bits);
     }
@@ -1248,13 +1268,13 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, int V, int n, int s0
       for (int it = 0; done < k && s0 + NT * it < s1; ++it) {
         const int s = s0 + tid + NT * it;
         uint32_t bits = 0;
-        const int b = slot_base<VEC>(s < s1 ? s : s1 - 1, V);
+        const int b = span.base(s < s1 ? s : s1 - 1);
         if (s < s1) {
           float v[VEC];
           slot_load<DT, VEC>(p, b, v);
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (b + e >= s * VEC && b + e < n && order_key(v[e]) == tau) bits |= 1u << e;
+            if (span.holds(s, b + e) && order_key(v[e]) == tau) bits |= 1u << e;
         }
         int run = __popc(bits);     // inclusive scan over the wavefront
 #pragma unroll
@@ -1311,7 +1331,7 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, int V, int n, int s0
 
 // One workgroup per row (or per part of a row): every element is read once, kUnroll 16-byte slots in flight per thread.
 // Four wavefronts where there are rows or parts enough to fill the chip (several workgroups a compute unit hide each
-// other's joins), sixteen where there are few.
+// other's joins), sixteen where there are few, one where there are many of moderate length.
 template <int DT, bool ENT, bool TOP, int NT>
 __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
   constexpr int VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
@@ -1325,11 +1345,11 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
     if (tid == 0 && part == 0 && a.log_prob) a.log_prob[row] = 0.f;
     return;
   }
-  const int n = row_size(a.r, row), V = a.r.V;
-  const int ns = (n + VEC - 1) / VEC;
-  const int per = ((ns + a.parts - 1) / a.parts + 15) & ~15;      // equal to 16 slots
-  const int s0 = part * per < ns ? part * per : ns, s1 = s0 + per < ns ? s0 + per : ns;
+  const int n = row_size(a.r, row);
   const char* p = a.r.x + row * a.r.ld * ES;
+  const Span<VEC> span(p, ES, a.r.V, n);
+  const int ns = span.slots, per = ((ns + a.parts - 1) / a.parts + 15) & ~15;      // equal to 16 slots
+  const int s0 = part * per < ns ? part * per : ns, s1 = s0 + per < ns ? s0 + per : ns;
   int gsz = (s1 - s0 + NT * kGroups - 1) / (NT * kGroups);    // slots per group of the selection: 1, 2 or whole rounds
   gsz = gsz <= 2 ? (gsz < 1 ? 1 : gsz) : (gsz + kUnroll - 1) / kUnroll * kUnroll;
   Online on;
@@ -1343,21 +1363,24 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
 #pragma unroll
     for (int q = 0; q < IN; ++q) {
       const int sq = sb + q * NT;
-      raw[q] = *(const Raw16*)(p + (int64_t)slot_base<VEC>(sq < s1 ? sq : sb, V) * ES);
+      raw[q] = *(const Raw16*)(p + (int64_t)span.base(sq < s1 ? sq : sb) * ES);
     }
 #pragma unroll
     for (int h = 0; h < IN; h += kUnroll) {
       const int s = sb + h * NT;
+      // the wavefront's first slot: a last round sums only as many slots a lane as it has
+      const int first = __builtin_amdgcn_readfirstlane(s);
+      const bool full = first + (kUnroll - 1) * NT < s1;
       float v[kUnroll * VEC];
 #pragma unroll
       for (int q = 0; q < kUnroll; ++q) {
         Elem<DT>::unpack(raw[h + q], v + q * VEC);
         const int sq = s + q * NT;
-        if (sq * VEC + VEC > n || sq >= s1) {       // the row's last slot, and past the end
-          const int b = slot_base<VEC>(sq < s1 ? sq : sb, V);
+        if (sq >= s1 || !span.whole(sq)) {       // the row's first and last slots, and past the end
+          const int b = span.base(sq);
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (sq >= s1 || b + e < sq * VEC || b + e >= n) v[q * VEC + e] = -INFINITY;
+            if (sq >= s1 || !span.holds(sq, b + e)) v[q * VEC + e] = -INFINITY;
         }
       }
       float mx;
@@ -1394,7 +1417,13 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
       } else {
         mx = max_of<kUnroll * VEC>(v, -INFINITY);
       }
-      on.template add<kUnroll * VEC, ENT>(v, mx, a.c);
+      if (full) {
+        on.template add<kUnroll * VEC, ENT>(v, mx, a.c);
+      } else {
+#pragma unroll
+        for (int q = 0; q < kUnroll; ++q)
+          if (first + q * NT < s1) on.template add<VEC, ENT>(v + q * VEC, max_of<VEC>(v + q * VEC, -INFINITY), a.c);
+      }
     }
   }
   if constexpr (TOP) {
@@ -1408,11 +1437,11 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
     float sum = 0.f;
     for (int s = s0 + h + NT * tid; s < s1; s += NT * NT) {
       float v[VEC];
-      const int b = slot_base<VEC>(s, V);
+      const int b = span.base(s);
       slot_load<DT, VEC>(p, b, v);
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (b + e >= s * VEC && b + e < n && v[e] < ref) sum += exp2_hw((v[e] - ref) * a.c);
+        if (span.holds(s, b + e) && v[e] < ref) sum += exp2_hw((v[e] - ref) * a.c);
     }
     return sum;
   });
@@ -1421,7 +1450,7 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
     if (tid == 0) a.part[row * a.parts + part] = f32x4{m, r, u, 0.f};
     if constexpr (TOP) {
       uint2* o = a.part_top + (row * a.parts + part) * a.top;
-      block_top<DT, VEC, NT>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m,
+      block_top<DT, VEC, NT>(top_sh, p, span, s0, s1, gsz, a.top, m, on.m,
                          [&](int rank, uint32_t key, int i) { o[rank] = make_uint2(key, (uint32_t)i); });
     }
     return;
@@ -1448,7 +1477,7 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
       }
       return;
     }
-    block_top<DT, VEC, NT>(top_sh, p, V, n, s0, s1, gsz, a.top, m, on.m, [&](int rank, uint32_t key, int i) {
+    block_top<DT, VEC, NT>(top_sh, p, span, s0, s1, gsz, a.top, m, on.m, [&](int rank, uint32_t key, int i) {
       a.top_idx[row * a.top + rank] = i;
       a.top_lp[row * a.top + rank] = i < 0 ? -INFINITY : (key_value(key) - m) - logs;
     });
@@ -1922,7 +1951,8 @@ void by_type(int dt, F f) {
   else f(std::integral_constant<int, DMV_F16>());
 }
 
-// Few rows: sixteen wavefronts to each, where four would have more than one round of loads.
+// Few rows: sixteen wavefronts to each, where four would have more than one round of loads.  (Eight for 300 to 1500 rows
+// gained nothing: 1024 x 50000 float16 with entropy and 8 alternatives took 38 us instead of 29.)
 bool wide_rows(int64_t groups, int V, int dt) { return groups <= 256 && V > kRowThreads * kUnroll * vec_elems(dt); }
 
 // Many rows that are not very long: a wavefront to each.
@@ -1933,15 +1963,14 @@ bool single_wave_rows(int64_t groups, int V, int dt) { return groups >= kSingleR
 int parts_of(int64_t rows, int V, int dt) {
   const int64_t rounds = ((int64_t)V + (int64_t)kChunkSlots * vec_elems(dt) - 1) / ((int64_t)kChunkSlots * vec_elems(dt));
   if (rounds <= 16) return 1;
-  int64_t parts = (1024 + rows - 1) / rows;
+  int64_t parts = (2048 + rows - 1) / rows;
   if (parts > rounds) parts = rounds;
   if (parts > kMaxParts) parts = kMaxParts;
   return parts < 1 ? 1 : (int)parts;
 }
-// slots per thread of the kernel that keeps a row in a workgroup's registers; 0: it does not fit
-constexpr int64_t kRowMinRows = 128;    // fewer rows: several workgroups per row
+// One workgroup to a row that fits its registers (16 slots a thread).
 int64_t row_slots(int V, int dt) { return ((int64_t)V + vec_elems(dt) - 1) / vec_elems(dt); }
-bool row_fits(int64_t rows, int V, int dt) { return rows >= kRowMinRows && row_slots(V, dt) <= 16 * 1024; }
+bool row_fits(int V, int dt) { return row_slots(V, dt) <= 16 * 1024; }
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
@@ -2090,7 +2119,7 @@ static int64_t loss_parts(const DmvCatRows* r) {
 extern "C" size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r) {
   if (check_rows(r) != DMV_OK || r->rows == 0) return 0;
   size_t n = up16((size_t)loss_parts(r) * sizeof(double));
-  if (r->V > kSmallMax && !row_fits(r->rows, r->V, r->dtype))
+  if (r->V > kSmallMax && !row_fits(r->V, r->dtype))
     n += (size_t)r->rows * (1 + parts_of(r->rows, r->V, r->dtype)) * sizeof(f32x4);
   return n;
 }
@@ -2129,7 +2158,7 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
         }
       });
     });
-  } else if (row_fits(r->rows, r->V, r->dtype)) {
+  } else if (row_fits(r->V, r->dtype)) {
     by_type(r->dtype, [&](auto dt) { launch_distill_row<decltype(dt)::value>(a, st); });
   } else {
     a.parts = parts_of(r->rows, r->V, r->dtype);
