@@ -1623,7 +1623,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_bwd_chunk(Bwd a) {
 }
 
 
-// The teacher's distribution over one row by a workgroup, entry j on thread j (k <= NT): p and log p of this thread's entry
+// The teacher's distribution over one row by a workgroup, entry j on thread j (the launch has k <= NT): p and log p of this thread's entry
 // (p = 0 where it does not count), its index (-1), and what holds for the row.
 struct TeacherEntry {
   float p, lp;
@@ -1632,7 +1632,6 @@ struct TeacherEntry {
 };
 template <int NT>
 __device__ __forceinline__ TeacherEntry teacher_row(const Teacher& t, int64_t row, int64_t rows, int n, BlockRed<NT>& red) {
-  static_assert(NT >= kMaxTeacher, "one entry per thread");
   TeacherEntry e{0.f, 0.f, -1, false, false};
   float x = -INFINITY;
   bool bad = false;
@@ -1698,27 +1697,34 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
     return;
   }
   const char* p = a.r.x + row * a.r.ld * ES;
+  const int n = row_size(a.r, row);
+  const Span<VEC> span(p, ES, V, V);
+  const int slots = span.slots;
+  // a wavefront takes part in as many of the NV rounds as it has slots
+  const int wave0 = __builtin_amdgcn_readfirstlane(tid);
+  auto has = [&](int q) { return wave0 + NT * q < slots; };
   u32x4 raw[NV];
 #pragma unroll
-  for (int q = 0; q < NV; ++q) {
-    const int s = tid + NT * q;
-    raw[q] = __builtin_bit_cast(u32x4, *(const Raw16*)(p + (uint32_t)(slot_base<VEC>(s < ns ? s : ns - 1, V) * ES)));
-  }
-  const int n = row_size(a.r, row);
+  for (int q = 0; q < NV; ++q)
+    if (has(q)) {
+      const int s = tid + NT * q;
+      raw[q] = __builtin_bit_cast(u32x4, *(const Raw16*)(p + (uint32_t)(span.base(s < slots ? s : slots - 1) * ES)));
+    }
   const TeacherEntry te = teacher_row<NT>(a.t, row, a.r.rows, n, red);
   const float xi = te.i >= 0 ? Elem<DT>::load(p, te.i) : 0.f;
-  // what does not count becomes -inf, once: past the row's size, and what a last slot shares with the one before it
+  // what does not count becomes -inf, once: past the row's size, and what a first or last slot shares with its neighbour
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    if (NT * (q + 1) * VEC <= n) continue;
+    if (!has(q)) break;
+    if ((q > 0 || span.lead == 0) && NT * (q + 1) * VEC - span.lead <= n) continue;      // a round of whole slots
     const int s = again(tid) + NT * q;
-    if (s * VEC + VEC > n) {
-      const int b = slot_base<VEC>(s < ns ? s : ns - 1, V);
+    if (s >= slots || !span.whole(s) || span.base(s) + VEC > n) {
+      const int b = span.base(s < slots ? s : slots - 1);
       float v[VEC];
       pass_over<DT>(raw[q], v);
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (b + e < s * VEC || b + e >= n) v[e] = -INFINITY;
+        if (!span.holds(s, b + e) || b + e >= n) v[e] = -INFINITY;
       Raw16 w;
       Elem<DT>::pack(v, w);
       raw[q] = __builtin_bit_cast(u32x4, w);
@@ -1727,6 +1733,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
   Online on;
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
+    if (!has(q)) break;
     float v[VEC];
     pass_over<DT>(raw[q], v);
     on.m = max_of<VEC>(v, on.m);
@@ -1734,6 +1741,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
   const float local = on.m == -INFINITY ? 0.f : on.m;
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
+    if (!has(q)) break;
     float v[VEC];
     pass_over<DT>(raw[q], v);
 #pragma unroll
@@ -1746,6 +1754,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
     if (h == tid) {
 #pragma unroll
       for (int q = 0; q < NV; ++q) {
+        if (!has(q)) break;
         float v[VEC];
         pass_over<DT>(raw[q], v);
 #pragma unroll
@@ -1779,13 +1788,18 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int s = again(tid) + NT * q;
-    if (s >= ns) break;
+    if (s >= slots) break;
     float v[VEC];
     pass_over<DT>(raw[q], v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = exp2_hw((v[e] - m) * a.t.c) * f;
-    if (s * VEC + VEC <= V) slot_store<DT, VEC>(out, s * VEC, v);
-    else chunk_store<DT>(out, s, V - VEC, v);
+    const int b = span.base(s);
+    if (span.whole(s)) slot_store<DT, VEC>(out, b, v);
+    else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (span.holds(s, b + e)) Elem<DT>::store(out, b + e, v[e]);
+    }
   }
   __syncthreads();          // the dense part before the teacher's categories are written again
   if (te.i >= 0 && !te.bad) Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te)));
@@ -1968,9 +1982,9 @@ int parts_of(int64_t rows, int V, int dt) {
   if (parts > kMaxParts) parts = kMaxParts;
   return parts < 1 ? 1 : (int)parts;
 }
-// One workgroup to a row that fits its registers (16 slots a thread).
+// One workgroup to a row that fits its registers (20 slots a thread of 1024).
 int64_t row_slots(int V, int dt) { return ((int64_t)V + vec_elems(dt) - 1) / vec_elems(dt); }
-bool row_fits(int V, int dt) { return row_slots(V, dt) <= 16 * 1024; }
+bool row_fits(int V, int dt) { return row_slots(V, dt) < 20 * 1024; }
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
@@ -1994,14 +2008,19 @@ void launch_fwd_rows(const Fwd& a, bool entropy, hipStream_t st) {
 
 template <int DT>
 void launch_distill_row(const Dist& a, hipStream_t st) {
-  const int64_t ns = row_slots(a.r.V, DT);
+  // (a row that starts between multiples of 16 bytes may have one slot more)
+  const bool aligned = (((uintptr_t)a.r.x | (uintptr_t)(a.r.ld * elem_size(DT))) & 15) == 0;
+  const int64_t ns = row_slots(a.r.V, DT) + (aligned ? 0 : 1);
   const dim3 grid((unsigned)a.r.rows);
-  if (ns <= 2 * 256) k_cat_distill_row<DT, 256, 2><<<grid, 256, 0, st>>>(a);
+  // (two wavefronts to the shortest: 16384 x 2500 bfloat16 54 us, by four 69; 20000 x 3000 float32 106 us, by four 94)
+  if (ns <= 5 * 128 && a.t.k <= 128) k_cat_distill_row<DT, 128, 5><<<grid, 128, 0, st>>>(a);
+  else if (ns <= 2 * 256) k_cat_distill_row<DT, 256, 2><<<grid, 256, 0, st>>>(a);
   else if (ns <= 4 * 256) k_cat_distill_row<DT, 256, 4><<<grid, 256, 0, st>>>(a);
   else if (ns <= 8 * 256) k_cat_distill_row<DT, 256, 8><<<grid, 256, 0, st>>>(a);
   else if (ns <= 16 * 256) k_cat_distill_row<DT, 256, 16><<<grid, 256, 0, st>>>(a);
   else if (ns <= 16 * 512) k_cat_distill_row<DT, 512, 16><<<grid, 512, 0, st>>>(a);
-  else k_cat_distill_row<DT, 1024, 16><<<grid, 1024, 0, st>>>(a);
+  else if (ns <= 16 * 1024) k_cat_distill_row<DT, 1024, 16><<<grid, 1024, 0, st>>>(a);
+  else k_cat_distill_row<DT, 1024, 20><<<grid, 1024, 0, st>>>(a);
 }
 
 }  // namespace
