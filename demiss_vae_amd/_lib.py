@@ -17,7 +17,6 @@ IN_PLAIN, IN_MASKED, IN_CONCAT, IN_CONCAT_MASKED = 0, 1, 2, 3
 GEN = {"normal": 0, "normal_with_eps": 1, "bern": 2, "bern_m1_p1": 3}
 Q_OWN, Q_STRATIFIED, Q_IMPUTATION = 0, 1, 2
 BOUND_LSE, BOUND_WEIGHTED, BOUND_PER_COMPONENT, TERMS_ONLY = 0, 1, 2, -1
-CAT_DTYPE = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
 CAT_MAX_TOP, CAT_MAX_TEACHER, CAT_SHORT_ROW = 64, 256, 2048
 E_BADARG, E_UNSUPPORTED, E_WORKSPACE = -1, -2, -3
 
@@ -154,7 +153,7 @@ SIGNATURES = {
     "dmv_cat_log_prob_ws_bytes": (_SZ, [C.POINTER(DmvCatRows), _I32]),
     "dmv_cat_log_prob": (C.c_int, [C.POINTER(DmvCatRows), _P, _P, _I32, _P, _P, _P, _P, _SZ, _P]),
     "dmv_cat_log_prob_backward": (C.c_int, [C.POINTER(DmvCatRows), _P, _P, _P, _I32, _P, _P, _P, _I64, _P]),
-    "dmv_cat_distill_ws_bytes": (_SZ, [C.POINTER(DmvCatRows)]),
+    "dmv_cat_distill_ws_bytes": (_SZ, [C.POINTER(DmvCatRows), _I32]),
     "dmv_cat_distill": (C.c_int, [C.POINTER(DmvCatRows), C.POINTER(DmvCatTeacher), _P, _P, _P, _P, _I64, _P, _SZ, _P]),
     "dmv_cat_distill_backward": (C.c_int, [C.POINTER(DmvCatRows), C.POINTER(DmvCatTeacher), _P, _I32, _P, _P, _I64, _P]),
     "dmv_lair_row_map": (C.c_int, [_I32, _I32, _I32, _P, _P, _P]),

@@ -44,6 +44,8 @@ def _rows(logits):
 
 def _per_row(t, lead, dtype, what, device, tail=()):
     """A per-row argument as a contiguous array that repeats over the leading dimensions: (tensor, period)."""
+    if t.dtype == dtype and t.device == device and (t.shape[:-1] if tail else t.shape) == lead and t.is_contiguous():
+        return t, t.numel() // tail[0] if tail else t.numel()
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the logits on {device}")
     if t.dtype != dtype:
@@ -51,7 +53,7 @@ def _per_row(t, lead, dtype, what, device, tail=()):
     shape = tuple(t.shape[:t.dim() - len(tail)])
     if len(shape) > len(lead):
         raise ValueError(f"{what} of shape {tuple(t.shape)} does not fit rows of shape {tuple(lead)}")
-    while shape and shape[0] == 1 and len(shape) > 0 and (len(shape) <= len(lead)):
+    while shape and shape[0] == 1:
         shape = shape[1:]
     if shape != tuple(lead[len(lead) - len(shape):]):
         try:
@@ -117,6 +119,10 @@ def _set_logits(r, logits, keep):
         keep.append(flat)
 
 
+def _like(logits):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format, requires_grad=False)
+
+
 def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
@@ -149,17 +155,19 @@ def _log_prob(dev, logits, r, keep, want_lp, entropy, top, want_stats):
     ent = torch.empty(lead, dtype=f32, device=dev) if entropy else None
     top_lp = torch.empty((*lead, top), dtype=f32, device=dev) if top else None
     top_idx = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty((r.rows, 4), dtype=f32, device=dev) if want_stats else None
+    n_stats = 4 * r.rows if want_stats else 0
     n_ws = lib.dmv_cat_log_prob_ws_bytes(C.byref(r), top) if r.V > L.CAT_SHORT_ROW else 0
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
-    L.check(lib.dmv_cat_log_prob(C.byref(r), L.addr(lp), L.addr(ent), top, L.addr(top_lp), L.addr(top_idx), L.addr(stats),
-                                 L.addr(ws), n_ws, _stream(dev)))
+    # the row statistics that the gradient reads, and behind them the workspace
+    stats = torch.empty(n_stats + n_ws // 4, dtype=f32, device=dev) if n_stats or n_ws else None
+    at = L.addr(stats)
+    L.check(lib.dmv_cat_log_prob(C.byref(r), L.addr(lp), L.addr(ent), top, L.addr(top_lp), L.addr(top_idx), at if n_stats else None,
+                                 at + 4 * n_stats if n_ws else None, n_ws, _stream(dev)))
     return lp, ent, top_lp, top_idx, stats
 
 
 @_on_device
 def _log_prob_backward(dev, logits, r, stats, g_lp, g_ent, top, top_idx, g_top):
-    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    d = _like(logits)
     L.check(L.lib().dmv_cat_log_prob_backward(C.byref(r), L.addr(stats), L.addr(g_lp), L.addr(g_ent), top, L.addr(top_idx),
                                               L.addr(g_top), L.addr(d), r.V, _stream(dev)))
     return d
@@ -214,12 +222,13 @@ def _distill(dev, logits, r, t, keep, training):
     _set_logits(r, logits, keep)
     per_row = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    d = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if training else None
-    stats = torch.empty((r.rows, 4), dtype=torch.float32, device=dev) if training and r.V > L.CAT_SHORT_ROW else None
-    n_ws = lib.dmv_cat_distill_ws_bytes(C.byref(r))
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-    L.check(lib.dmv_cat_distill(C.byref(r), C.byref(t), L.addr(per_row), L.addr(loss), L.addr(stats), L.addr(d), r.V, L.addr(ws), n_ws,
-                                _stream(dev)))
+    d = _like(logits) if training else None
+    n_stats = 4 * r.rows if training and r.V > L.CAT_SHORT_ROW else 0
+    n_ws = lib.dmv_cat_distill_ws_bytes(C.byref(r), t.k)
+    stats = torch.empty(n_stats + n_ws // 4, dtype=torch.float32, device=dev) if n_stats or n_ws else None      # as in _log_prob
+    at = L.addr(stats)
+    L.check(lib.dmv_cat_distill(C.byref(r), C.byref(t), per_row.data_ptr(), loss.data_ptr(), at if n_stats else None, L.addr(d), r.V,
+                                at + 4 * n_stats if n_ws else None, n_ws, _stream(dev)))
     return loss, per_row, stats, d
 
 
@@ -227,7 +236,7 @@ def _distill(dev, logits, r, t, keep, training):
 def _distill_backward(dev, logits, r, t, g, stats, d):
     unless_one = d is not None
     if d is None:
-        d = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        d = _like(logits)
     L.check(L.lib().dmv_cat_distill_backward(C.byref(r), C.byref(t), L.addr(g), unless_one, L.addr(stats), L.addr(d), r.V, _stream(dev)))
     return d
 

@@ -2126,18 +2126,22 @@ template <typename T>
 bool lone_group(int64_t rows, int k) {
   return rows <= 4 * (kLoneThreads / T::L) && (size_t)(kLoneThreads / T::L) * k * sizeof(Entry) <= 48 * 1024;
 }
-static int64_t loss_parts(const DmvCatRows* r) {
+// shares of the loss that a launch leaves to the sum; 0: it forms the loss itself
+static int64_t loss_parts(const DmvCatRows* r, int k) {
   int64_t n = r->rows;
   if (r->V <= kSmallMax)
     by_type(r->dtype, [&](auto dt) {
-      small_tile<decltype(dt)::value>(r->V, [&](auto t) { n = decltype(t)::groups(r->rows); });
+      small_tile<decltype(dt)::value>(r->V, [&](auto t) {
+        typedef decltype(t) T;
+        n = lone_group<T>(r->rows, k) ? 0 : T::groups(r->rows);
+      });
     });
   return n;
 }
 
-extern "C" size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r) {
-  if (check_rows(r) != DMV_OK || r->rows == 0) return 0;
-  size_t n = up16((size_t)loss_parts(r) * sizeof(double));
+extern "C" size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r, int32_t k) {
+  if (check_rows(r) != DMV_OK || r->rows == 0 || k < 1 || k > kMaxTeacher) return 0;
+  size_t n = up16((size_t)loss_parts(r, k) * sizeof(double));
   if (r->V > kSmallMax && !row_fits(r->V, r->dtype))
     n += (size_t)r->rows * (1 + parts_of(r->rows, r->V, r->dtype)) * sizeof(f32x4);
   return n;
@@ -2157,8 +2161,9 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
   rc = check_teacher(r, t);
   if (rc != DMV_OK) return rc;
   if (((uintptr_t)stats & 15) != 0 || (d_logits && ((uintptr_t)d_logits % elem_size(r->dtype)) != 0)) return DMV_E_BADARG;
-  if (!ws || ((uintptr_t)ws & 15) != 0 || ws_bytes < dmv_cat_distill_ws_bytes(r)) return DMV_E_WORKSPACE;
-  const int64_t n_loss = loss_parts(r);
+  const size_t need = dmv_cat_distill_ws_bytes(r, t->k);
+  if (need && (!ws || ((uintptr_t)ws & 15) != 0 || ws_bytes < need)) return DMV_E_WORKSPACE;
+  const int64_t n_loss = loss_parts(r, t->k);
   Dist a = dist_of(r, t);
   a.per_row = per_row;
   a.loss_part = (double*)ws;

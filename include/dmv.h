@@ -561,7 +561,7 @@ int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats, const flo
  * makes the row's loss and gradient NaN; categories of probability 0 under q with p > 0 make the loss inf.  The sum of
  * the loss has a fixed order and is held in 64 bits.
  * stats: needed by the backward call for V > DMV_CAT_SHORT_ROW ([rows][4], 16-byte aligned), nullable.
- * ws: dmv_cat_distill_ws_bytes bytes, 16-byte aligned. */
+ * ws: dmv_cat_distill_ws_bytes bytes, 16-byte aligned (may be 0). */
 typedef struct DmvCatTeacher {
   const void* logits;     /* [period][k] */
   const int64_t* index;   /* [period][k] */
@@ -572,7 +572,7 @@ typedef struct DmvCatTeacher {
   int64_t w_period;
   float temperature;      /* > 0 */
 } DmvCatTeacher;
-size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r);
+size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r, int32_t k);
 int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, float* per_row, float* loss, float* stats, void* d_logits,
                     int64_t ld_d, void* ws, size_t ws_bytes, void* stream);
 /* d_logits = *gscale times the gradient of loss, from the logits again (one rounding).  unless_one: return at once, on the

@@ -96,7 +96,7 @@ def test_entry_points_refuse_rows(kw, code):
     assert lib.dmv_cat_log_prob_backward(r, FAKE, FAKE, None, 0, None, None, FAKE, 1 << 40, None) == code
     assert lib.dmv_cat_distill(r, t, FAKE, FAKE, None, None, 0, FAKE, 1 << 40, None) == code
     assert lib.dmv_cat_distill_backward(r, t, FAKE, 0, FAKE, FAKE, 1 << 40, None) == code
-    assert lib.dmv_cat_log_prob_ws_bytes(r, 1) == 0 and lib.dmv_cat_distill_ws_bytes(r) == 0
+    assert lib.dmv_cat_log_prob_ws_bytes(r, 1) == 0 and lib.dmv_cat_distill_ws_bytes(r, 2) == 0
 
 
 @pytest.mark.parametrize("args, code", [
@@ -145,9 +145,10 @@ def test_distill_entry_refuses_teacher(kw, code):
 
 def test_distill_entry_refuses_outputs_and_workspace():
     lib = L.lib()
-    r, t = C.byref(_rows()), C.byref(_teacher())
-    need = lib.dmv_cat_distill_ws_bytes(r)
-    assert need >= 8
+    r, t = C.byref(_rows(rows=100000)), C.byref(_teacher())
+    need = lib.dmv_cat_distill_ws_bytes(r, 2)
+    assert need >= 8 and need % 16 == 0
+    assert lib.dmv_cat_distill_ws_bytes(C.byref(_rows()), 2) == 0           # a small launch forms the loss itself
     call = lambda loss=FAKE, stats=None, d=None, ld=8, ws=FAKE, n=need: lib.dmv_cat_distill(r, t, None, loss, stats, d, ld, ws, n, None)  # noqa: E731
     assert call(loss=None) == BAD and call(d=FAKE, ld=7) == BAD and call(d=FAKE + 1) == BAD and call(stats=FAKE + 4) == BAD
     assert call(ws=None) == WORKSPACE and call(n=need - 1) == WORKSPACE and call(ws=FAKE + 8) == WORKSPACE
