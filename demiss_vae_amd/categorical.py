@@ -105,6 +105,8 @@ def _row_args(logits, X, M, sizes):
         keep.append(M)
     if sizes is not None:
         _integers(sizes, "sizes")
+        if sizes.dtype != torch.int32:
+            sizes = sizes.clamp(0, r.V)
         sizes, r.size_period = _per_row(sizes, lead, torch.int32, "sizes", dev)
         r.sizes = sizes.data_ptr()
         keep.append(sizes)
@@ -137,13 +139,15 @@ def _on_device(f):
     return call
 
 
-def _backward(f):
-    """A backward pass in terms of kernel launches: fine as it is, unless autograd records it (create_graph=True)."""
-    once = torch.autograd.function.once_differentiable(f)
+class _Once(torch.autograd.Function):
+    """A gradient that autograd records (create_graph=True): it may be used, not differentiated."""
+    @staticmethod
+    def forward(ctx, d, logits):
+        return d.view_as(d)
 
-    def backward(ctx, *grads):
-        return once(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
-    return staticmethod(backward)
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("the categorical operators have no second derivative")
 
 
 @_on_device
@@ -184,13 +188,15 @@ class _LogProb(torch.autograd.Function):
             ctx.mark_non_differentiable(top_idx)
         return lp, ent, top_lp, top_idx
 
-    @_backward
+    @staticmethod
     def backward(ctx, g_lp, g_ent, g_top, _):
         d = None
         if g_lp is not None or g_ent is not None or g_top is not None:
             logits, stats, top_idx = ctx.saved_tensors
             g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
             d = _log_prob_backward(logits.device, logits, ctx.r, stats, g_lp, g_ent, ctx.top, top_idx, g_top)
+            if torch.is_grad_enabled():
+                d = _Once.apply(d, logits)
         return d, None, None, None, None, None
 
 
@@ -251,7 +257,7 @@ class _Distill(torch.autograd.Function):
         ctx.mark_non_differentiable(per_row)
         return loss, per_row
 
-    @_backward
+    @staticmethod
     def backward(ctx, g, _):
         if g is None:
             return None, None, None, None
@@ -259,7 +265,8 @@ class _Distill(torch.autograd.Function):
         # the forward pass has written the gradient for g = 1 (a loss that is not scaled further): any other g forms it
         # again from the logits, on the device; a second backward pass has a gradient of its own
         d, ctx.d = ctx.d, None
-        return _distill_backward(logits.device, logits, ctx.r, ctx.t, g, stats, d), None, None, None
+        d = _distill_backward(logits.device, logits, ctx.r, ctx.t, g, stats, d)
+        return _Once.apply(d, logits) if torch.is_grad_enabled() else d, None, None, None
 
 
 def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None, temperature=1.0):
@@ -277,8 +284,8 @@ def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None
     leaves past a row's categories); a category given twice counts twice."""
     _check_logits(logits)
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature = {temperature}: a positive number")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature = {temperature}: 1e-30 .. 1e30")
     if top_logits.shape != top_index.shape or top_logits.dim() < 1:
         raise ValueError(f"top_logits {tuple(top_logits.shape)} and top_index {tuple(top_index.shape)}: one shape [..., k]")
     if top_logits.dtype not in _DTYPES:

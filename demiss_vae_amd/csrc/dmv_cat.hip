@@ -1915,7 +1915,6 @@ __global__ void __launch_bounds__(kLossThreads) k_cat_loss(const double* part, i
 }
 
 // ------------------------------------------------------------------------------------------ host side
-constexpr int64_t kMaxGrid = 0x7fffffffll;
 
 int check_rows(const DmvCatRows* r) {
   if (!r || r->rows < 0 || r->V < 1 || r->ld < 0) return DMV_E_BADARG;
@@ -1923,10 +1922,11 @@ int check_rows(const DmvCatRows* r) {
   if (r->rows == 0) return DMV_OK;
   if (!r->logits || ((uintptr_t)r->logits % elem_size(r->dtype)) != 0) return DMV_E_BADARG;
   if ((r->X && r->x_period < 1) || (r->M && r->m_period < 1) || (r->sizes && r->size_period < 1)) return DMV_E_BADARG;
-  // a workgroup per row and part, and slot numbers in 32 bits with room for a chunk
-  if (r->rows > kMaxGrid / kMaxParts || r->V > 0x7fffffff - (1 << 20)) return DMV_E_UNSUPPORTED;
+  // row numbers of short rows and threads of a launch in 32 bits, slot numbers in 32 bits with room for a chunk
+  if (r->rows >= (int64_t)1 << 26 || r->V > 0x7fffffff - (1 << 20)) return DMV_E_UNSUPPORTED;
   return DMV_OK;
 }
+bool fits_grid(int64_t groups, int threads) { return groups * threads < (int64_t)1 << 32; }
 Rows rows_of(const DmvCatRows* r) {
   return Rows{(const char*)r->logits, r->ld, r->rows, r->V, r->X, r->M, r->sizes, r->x_period, r->m_period, r->size_period};
 }
@@ -1939,6 +1939,15 @@ struct Tile {
   static int64_t groups(int64_t rows) { return (rows + kSmallThreads / L - 1) / (kSmallThreads / L); }
 };
 template <int DT, typename F>
+void wide_tile(int V, int lanes, F f) {
+  constexpr int N = Elem<DT>::N, S = 32 / N;
+  const int ns = (V + N - 1) / N;
+  if (lanes <= 8 && ns <= 8 * S) return f(Tile<DT, N, 8, S>());
+  if (ns <= 16 * S) return f(Tile<DT, N, 16, S>());
+  if (ns <= 32 * S) return f(Tile<DT, N, 32, S>());
+  return f(Tile<DT, N, 64, S>());
+}
+template <int DT, typename F>
 void small_tile(int V, F f) {
   constexpr int N = Elem<DT>::N, S = 32 / N;
   const int ns = (V + N - 1) / N;
@@ -1948,10 +1957,14 @@ void small_tile(int V, F f) {
   if (ns <= 16) return f(Tile<DT, N, 4, 4>());
   if constexpr (S == 8)
     if (ns <= 32) return f(Tile<DT, N, 4, 8>());
-  if (ns <= 8 * S) return f(Tile<DT, N, 8, S>());
-  if (ns <= 16 * S) return f(Tile<DT, N, 16, S>());
-  if (ns <= 32 * S) return f(Tile<DT, N, 32, S>());
-  return f(Tile<DT, N, 64, S>());
+  wide_tile<DT>(V, 8, f);
+}
+// ... for distillation: a lane group's k teacher entries are in LDS, which 256 / L groups share
+template <int DT, typename F>
+void teacher_tile(int V, int k, F f) {
+  if (k <= 64) return small_tile<DT>(V, f);
+  if (V < Elem<DT>::N) return f(Tile<DT, 1, 16, 1>());
+  wide_tile<DT>(V, k <= 128 ? 8 : 16, f);
 }
 // LDS of a workgroup's teacher entries
 template <typename T>
@@ -2063,6 +2076,7 @@ extern "C" int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* ent
     return DMV_OK;
   }
   a.parts = parts_of(r->rows, r->V, r->dtype);
+  if (!fits_grid(r->rows * a.parts, single_wave_rows(r->rows, r->V, r->dtype) ? 64 : kRowThreads)) return DMV_E_UNSUPPORTED;
   if (a.parts > 1) {
     if (!ws || ws_bytes < dmv_cat_log_prob_ws_bytes(r, top)) return DMV_E_WORKSPACE;
     a.part = (f32x4*)ws;
@@ -2100,7 +2114,7 @@ extern "C" int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats
     return DMV_OK;
   }
   a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
-  if (r->rows > kMaxGrid / a.chunks) return DMV_E_UNSUPPORTED;
+  if (!fits_grid(r->rows * a.chunks, kRowThreads)) return DMV_E_UNSUPPORTED;
   by_type(r->dtype, [&](auto dt) {
     k_cat_bwd_chunk<decltype(dt)::value><<<(unsigned)(r->rows * a.chunks), kRowThreads, 0, st>>>(a);
   });
@@ -2111,7 +2125,7 @@ extern "C" int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats
 static int check_teacher(const DmvCatRows* r, const DmvCatTeacher* t) {
   if (!t || t->k < 1 || !t->logits || !t->index || t->period < 1 || (t->weight && t->w_period < 1)) return DMV_E_BADARG;
   if (t->dtype < DMV_F32 || t->dtype > DMV_F16 || t->k > kMaxTeacher) return DMV_E_UNSUPPORTED;
-  if (((uintptr_t)t->logits % elem_size(t->dtype)) != 0 || !(t->temperature > 0.f) || !(t->temperature <= 3.4e38f)) return DMV_E_BADARG;
+  if (((uintptr_t)t->logits % elem_size(t->dtype)) != 0 || !(t->temperature >= 1e-30f && t->temperature <= 1e30f)) return DMV_E_BADARG;
   return DMV_OK;
 }
 static Dist dist_of(const DmvCatRows* r, const DmvCatTeacher* t) {
@@ -2131,7 +2145,7 @@ static int64_t loss_parts(const DmvCatRows* r, int k) {
   int64_t n = r->rows;
   if (r->V <= kSmallMax)
     by_type(r->dtype, [&](auto dt) {
-      small_tile<decltype(dt)::value>(r->V, [&](auto t) {
+      teacher_tile<decltype(dt)::value>(r->V, k, [&](auto t) {
         typedef decltype(t) T;
         n = lone_group<T>(r->rows, k) ? 0 : T::groups(r->rows);
       });
@@ -2172,7 +2186,7 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
   a.ld_d = ld_d;
   if (r->V <= kSmallMax) {
     by_type(r->dtype, [&](auto dt) {
-      small_tile<decltype(dt)::value>(r->V, [&](auto tile) {
+      teacher_tile<decltype(dt)::value>(r->V, t->k, [&](auto tile) {
         typedef decltype(tile) T;
         if (lone_group<T>(r->rows, t->k)) {
           a.loss = loss;
@@ -2182,6 +2196,8 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
         }
       });
     });
+  } else if (!fits_grid(r->rows, row_slots(r->V, r->dtype) < 5 * 128 && t->k <= 128 ? 128 : kRowThreads)) {
+    return DMV_E_UNSUPPORTED;
   } else if (row_fits(r->V, r->dtype)) {
     by_type(r->dtype, [&](auto dt) { launch_distill_row<decltype(dt)::value>(a, st); });
   } else {
@@ -2224,7 +2240,7 @@ extern "C" int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher
   by_type(r->dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (r->V <= kSmallMax) {
-      small_tile<DT>(r->V, [&](auto tile) {
+      teacher_tile<DT>(r->V, t->k, [&](auto tile) {
         typedef decltype(tile) T;
         k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kSmallThreads><<<(unsigned)T::groups(r->rows), kSmallThreads, small_lds<T>(t->k), st>>>(a);
       });

@@ -520,7 +520,8 @@ int dmv_grid_divergences(int32_t gen_dist, int32_t D, int32_t Zd, int64_t Nz, co
  *   their logits hold; clamped to 0..V).
  * A row without any category of non-zero probability (size 0, or all logits -inf) has entropy 0, log-probability -inf,
  * no alternatives and a zero gradient.  NaN or +inf among a row's logits makes its outputs NaN (alternatives -1); a given
- * category outside the row's, where it is seen, makes that row's log-probability and gradient NaN. */
+ * category outside the row's, where it is seen, makes that row's log-probability and gradient NaN.
+ * Limits (DMV_E_UNSUPPORTED): fewer than 2^26 rows (2^24 where V > DMV_CAT_SHORT_ROW), V below 2^31 - 2^20. */
 enum { DMV_F32 = 0, DMV_BF16 = 1, DMV_F16 = 2 };
 #define DMV_CAT_MAX_TOP 64
 #define DMV_CAT_MAX_TEACHER 256
@@ -570,7 +571,7 @@ typedef struct DmvCatTeacher {
   int32_t dtype;
   const float* weight;
   int64_t w_period;
-  float temperature;      /* > 0 */
+  float temperature;      /* 1e-30 .. 1e30 */
 } DmvCatTeacher;
 size_t dmv_cat_distill_ws_bytes(const DmvCatRows* r, int32_t k);
 int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, float* per_row, float* loss, float* stats, void* d_logits,

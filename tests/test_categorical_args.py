@@ -85,7 +85,7 @@ BAD, UNSUPPORTED, WORKSPACE = L.E_BADARG, L.E_UNSUPPORTED, L.E_WORKSPACE
 ROWS_REFUSED = [(dict(rows=-1), BAD), (dict(V=0), BAD), (dict(ld=-1), BAD), (dict(logits=None), BAD), (dict(logits=FAKE + 2), BAD),
                 (dict(dtype=1, logits=FAKE + 1), BAD), (dict(x_period=0), BAD), (dict(M=FAKE, m_period=0), BAD),
                 (dict(sizes=FAKE, size_period=0), BAD), (dict(dtype=3), UNSUPPORTED), (dict(dtype=-1), UNSUPPORTED),
-                (dict(rows=1 << 31), UNSUPPORTED), (dict(V=0x7fffffff), UNSUPPORTED)]
+                (dict(rows=1 << 26), UNSUPPORTED), (dict(V=0x7fffffff), UNSUPPORTED)]
 
 
 @pytest.mark.parametrize("kw, code", ROWS_REFUSED)
@@ -134,13 +134,23 @@ def test_backward_entry_refuses(args, code):
 
 @pytest.mark.parametrize("kw, code", [
     (dict(logits=None), BAD), (dict(index=None), BAD), (dict(period=0), BAD), (dict(k=0), BAD), (dict(k=257), UNSUPPORTED),
-    (dict(dtype=5), UNSUPPORTED), (dict(temperature=0.0), BAD), (dict(temperature=-1.0), BAD), (dict(temperature=float("nan")), BAD),
+    (dict(dtype=5), UNSUPPORTED), (dict(temperature=0.0), BAD), (dict(temperature=-1.0), BAD), (dict(temperature=1e-40), BAD), (dict(temperature=1e38), BAD), (dict(temperature=float("nan")), BAD),
     (dict(weight=FAKE, w_period=0), BAD), (dict(logits=FAKE + 1), BAD)])
 def test_distill_entry_refuses_teacher(kw, code):
     lib = L.lib()
     t = C.byref(_teacher(**kw))
     assert lib.dmv_cat_distill(C.byref(_rows()), t, FAKE, FAKE, None, None, 0, FAKE, 1 << 30, None) == code
     assert lib.dmv_cat_distill_backward(C.byref(_rows()), t, FAKE, 0, FAKE, FAKE, 8, None) == code
+
+
+def test_entries_refuse_launches_beyond_the_grid():
+    """2^32 threads and more in one launch"""
+    lib = L.lib()
+    r = C.byref(_rows(rows=(1 << 24) + 5, V=70000, ld=70000))
+    assert lib.dmv_cat_log_prob(r, FAKE, None, 0, None, None, None, None, 0, None) == UNSUPPORTED
+    assert lib.dmv_cat_log_prob_backward(r, FAKE, FAKE, None, 0, None, None, FAKE, 70000, None) == UNSUPPORTED
+    need = lib.dmv_cat_distill_ws_bytes(r, 2)
+    assert lib.dmv_cat_distill(r, C.byref(_teacher()), None, FAKE, None, None, 0, FAKE, need, None) == UNSUPPORTED
 
 
 def test_distill_entry_refuses_outputs_and_workspace():

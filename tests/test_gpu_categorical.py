@@ -233,6 +233,7 @@ def test_broadcast_shapes(V):
         sizes = torch.full(shape, V, dtype=torch.int64, device="cuda")
         check_log_prob(x, X=X, M=M, sizes=sizes, entropy=True)
         check_log_prob(x, X=X.to(torch.int32))
+    check_log_prob(x, X=ints(V, (4,)), sizes=torch.tensor(2 ** 40, device="cuda").expand(4), entropy=True)
     check_log_prob(make((V,), torch.float32), X=ints(V, ()), entropy=True, top=2, grads=True)      # one row without leading dimensions
 
 
@@ -561,6 +562,49 @@ def test_distill_entries(V, rows, dtype):
     loss, per_row = dmv.distill_top_logits(zz, t, idx, sizes=sizes, weight=w, temperature=0.5)
     (dy,) = torch.autograd.grad(loss, zz)
     assert torch.equal(per_row, a[1]) and torch.equal(dy, a[2])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [2, 7, 30, 100, 128, 200, 256, 700, 3000, 70000])
+@pytest.mark.parametrize("k", [65, 129, 256])
+@pytest.mark.parametrize("rows", [3, 700])
+def test_distill_many_entries(V, k, rows, dtype):
+    """as many entries as may be given, more than there are categories: most of them given several times, some empty"""
+    rows = min(rows, 20_000_000 // V)
+    x = make((rows, V), dtype, seed=V)
+    idx = ints(V, (rows, k), seed=k)
+    idx[rand((rows, k), 6) < 0.1] = -1
+    check_distill(x, make((rows, k), torch.float32, seed=k), idx, weight=rand((rows,)) + 0.1, T=1.5)
+
+
+def test_temperatures():
+    x = make((5, 900), torch.float32, seed=2)
+    t, idx = teacher_of(x, 9)
+    for T in (0.05, 0.7, 30.0, 1e4):
+        check_distill(x, t, idx, T=T)
+    for T in (1e-30, 1e30):
+        loss, per_row = dmv.distill_top_logits(x, t, idx, temperature=T)
+        assert not bool(per_row.isnan().any())
+
+
+@pytest.mark.parametrize("V", [40, 5000])
+def test_saved_logits_and_second_derivatives(V):
+    x = make((4, V), torch.float32)
+    X = ints(V, (4,))
+    t, idx = teacher_of(x, 3)
+    for f in (lambda z: dmv.categorical_log_prob(z, X).log_prob.sum(), lambda z: dmv.distill_top_logits(z, t, idx)[0]):
+        z = x.clone().requires_grad_()
+        y = 1.0 * z
+        loss = f(y)
+        with torch.no_grad():
+            y.add_(1.0)                                # written over after the forward pass
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        (g,) = torch.autograd.grad(f(z), z, create_graph=True)
+        (want,) = torch.autograd.grad(f(z), z)
+        assert torch.equal(g.detach(), want)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            g.sum().backward()
 
 
 @pytest.mark.parametrize("V", [6, 1000, 2000, 66000])
