@@ -671,6 +671,10 @@ __device__ __forceinline__ void small_sorted(const float* o, int V, int lane, in
   for (int j = E * L + lane; j < k; j += L) emit(j, -INFINITY, -1);
 }
 
+// Short rows, forward.  Bound by the vector units and not by memory: of 706 instructions that a wavefront takes for eight rows
+// of 256 bfloat16 with entropy and 4 alternatives, the passes over the elements (unpack, maximum, exponential, two sums)
+// are 350.  100352 such rows: 20.4 us (2.8 TB/s); without alternatives and entropy 13 us (4.0 TB/s); 200000 x 100 float32
+// 14.4 us (5.5 TB/s).
 enum { kNoTop = 0, kRanked = 1, kSorted = 2 };
 template <int DT, int VEC, int L, int SL, bool ENT, int TOP>
 __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
@@ -1331,7 +1335,10 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& spa
 
 // One workgroup per row (or per part of a row): every element is read once, kUnroll 16-byte slots in flight per thread.
 // Four wavefronts where there are rows or parts enough to fill the chip (several workgroups a compute unit hide each
-// other's joins), sixteen where there are few, one where there are many of moderate length.
+// other's joins), sixteen where there are few, one where there are many of moderate length.  Measured: 2048 x 65536
+// bfloat16, log-probability alone 54 us (5.0 TB/s), with entropy and 8 alternatives 66 us (4.1 TB/s; the vector units are
+// 83 % busy); float32 92 us (5.8 TB/s) and 101 us; 8192 x 4096 bfloat16 15 and 26 us; 50 x 50000 float32 with 64
+// alternatives 15 us, bound by the latency of its phases.  Loading a round ahead gained nothing.
 template <int DT, bool ENT, bool TOP, int NT>
 __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
   constexpr int VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
@@ -1567,7 +1574,8 @@ __device__ __forceinline__ void chunk_store(char* out, int s, int base, const fl
   }
 }
 
-// Gradient of long rows: a workgroup per chunk of a row (kChunkSlots slots), the row's statistics are known.
+// Gradient of long rows: a workgroup per chunk of a row (kChunkSlots slots), the row's statistics are known.  One read and one
+// write of the row: 1024 x 50001 float16 36 us (5.7 TB/s), 2048 x 65536 bfloat16 99 us (5.4 TB/s), as fast as a copy.
 constexpr int kChunkSlots = kRowThreads * kUnroll;
 template <int DT>
 __global__ void __launch_bounds__(kRowThreads) k_cat_bwd_chunk(Bwd a) {
@@ -1672,7 +1680,10 @@ __device__ __forceinline__ float share_of(const SparseShared& sh, int k, const T
   return same > 1 ? logf(p) : e.lp;
 }
 
-// Loss and gradient of a row that fits the registers of one workgroup (NV slots per thread): the row is read once.
+// Loss and gradient of a row that fits the registers of one workgroup (NV slots per thread): the row is read once.  2048 x
+// 65536 bfloat16 with 32 entries 118 us (4.5 TB/s read and written; two workgroups of 512 a compute unit, one of 1024 took
+// 136), 4096 x 32000 106 us (5.0 TB/s), 1024 x 65536 float32 122 us (4.4 TB/s: one workgroup of 1024 a compute unit, whose
+// loads, sums and stores do not overlap).
 template <int DT, int NT, int NV>
 __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
   constexpr int VEC = Elem<DT>::N, ES = sizeof(typename Elem<DT>::type);
@@ -2135,10 +2146,11 @@ static Dist dist_of(const DmvCatRows* r, const DmvCatTeacher* t) {
   a.chunks = a.parts = 1;
   return a;
 }
-// A small launch: one workgroup does all rows in a few rounds, and the loss.
+// A small launch: one workgroup does all rows in two rounds at most, and the loss.  (64 x 1000 float32, two rounds: 15.6 us on
+// the GPU instead of 6.1 + 1.6, but a launch less of the host's 90 us a step; each further round takes 6 us more.)
 template <typename T>
 bool lone_group(int64_t rows, int k) {
-  return rows <= 4 * (kLoneThreads / T::L) && (size_t)(kLoneThreads / T::L) * k * sizeof(Entry) <= 48 * 1024;
+  return rows <= 2 * (kLoneThreads / T::L) && (size_t)(kLoneThreads / T::L) * k * sizeof(Entry) <= 48 * 1024;
 }
 // shares of the loss that a launch leaves to the sum; 0: it forms the loss itself
 static int64_t loss_parts(const DmvCatRows* r, int k) {
