@@ -156,6 +156,7 @@ SIGNATURES = {
     "dmv_cat_distill_ws_bytes": (_SZ, [C.POINTER(DmvCatRows), _I32]),
     "dmv_cat_distill": (C.c_int, [C.POINTER(DmvCatRows), C.POINTER(DmvCatTeacher), _P, _P, _P, _P, _I64, _P, _SZ, _P]),
     "dmv_cat_distill_backward": (C.c_int, [C.POINTER(DmvCatRows), C.POINTER(DmvCatTeacher), _P, _I32, _P, _P, _I64, _P]),
+    "dmv_capture_id": (_U64, [_P]),
     "dmv_lair_row_map": (C.c_int, [_I32, _I32, _I32, _P, _P, _P]),
     "dmv_dropout_masks": (C.c_int, [_P, _I64, _F, _U64, _U64, _P, _P]),
     "dmv_clock_watch": (C.c_int, [_I64, _P, _P]),

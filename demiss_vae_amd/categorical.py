@@ -72,8 +72,8 @@ def _check_logits(logits):
         raise ValueError("logits: a tensor [..., V]")
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits of type {logits.dtype}: float32, bfloat16 or float16")
-    if logits.shape[-1] < 1:
-        raise ValueError("logits without categories")
+    if not 1 <= logits.shape[-1] < 2 ** 31:
+        raise ValueError(f"logits of {logits.shape[-1]} categories: 1 .. 2^31 - 1")
 
 
 def _need_gpu(logits):
@@ -106,7 +106,7 @@ def _row_args(logits, X, M, sizes):
     if sizes is not None:
         _integers(sizes, "sizes")
         if sizes.dtype != torch.int32:
-            sizes = sizes.clamp(0, r.V)
+            sizes = sizes.to(torch.int64).clamp(0, r.V)
         sizes, r.size_period = _per_row(sizes, lead, torch.int32, "sizes", dev)
         r.sizes = sizes.data_ptr()
         keep.append(sizes)
@@ -121,12 +121,39 @@ def _set_logits(r, logits, keep):
         keep.append(flat)
 
 
+def _keep(ctx, logits, r, keep):
+    """What a backward pass needs of a call's arguments.  Its arrays are held here, and their versions, because pointers to
+    them are: saved tensors may come back from elsewhere, and may not have been made for saving (a teacher's, say)."""
+    ctx.r, ctx.keep, ctx.versions = r, keep, _versions(keep)
+    ctx.in_place = r.logits == logits.data_ptr()
+
+
+def _versions(keep):
+    return [0 if t.is_inference() else t._version for t in keep]
+
+
+def _kept(ctx, logits):
+    """The call's rows for its backward pass, with the saved logits where they are now; and what has to stay alive."""
+    if _versions(ctx.keep) != ctx.versions:
+        raise RuntimeError("a tensor that the gradient of a categorical operator needs (X, M, sizes, weight or the teacher's) "
+                           "was modified in place after the forward call")
+    if not ctx.in_place or ctx.r.logits == logits.data_ptr():
+        return ctx.r, None
+    r, moved = L.DmvCatRows.from_buffer_copy(ctx.r), []
+    _set_logits(r, logits, moved)
+    return r, moved
+
+
 def _like(logits):
     return torch.empty_like(logits, memory_format=torch.contiguous_format, requires_grad=False)
 
 
 def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _capture(device):
+    return L.lib().dmv_capture_id(_stream(device))
 
 
 def _on_device(f):
@@ -181,7 +208,8 @@ class _LogProb(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, r, keep, want_lp, entropy, top):
         lp, ent, top_lp, top_idx, stats = _log_prob(logits.device, logits, r, keep, want_lp, entropy, top, True)
-        ctx.r, ctx.keep, ctx.top = r, keep, top
+        _keep(ctx, logits, r, keep)
+        ctx.top = top
         ctx.save_for_backward(logits, stats, top_idx)
         ctx.set_materialize_grads(False)
         if top:
@@ -194,7 +222,8 @@ class _LogProb(torch.autograd.Function):
         if g_lp is not None or g_ent is not None or g_top is not None:
             logits, stats, top_idx = ctx.saved_tensors
             g_lp, g_ent, g_top = (None if g is None else g.contiguous() for g in (g_lp, g_ent, g_top))
-            d = _log_prob_backward(logits.device, logits, ctx.r, stats, g_lp, g_ent, ctx.top, top_idx, g_top)
+            r, moved = _kept(ctx, logits)
+            d = _log_prob_backward(logits.device, logits, r, stats, g_lp, g_ent, ctx.top, top_idx, g_top)
             if torch.is_grad_enabled():
                 d = _Once.apply(d, logits)
         return d, None, None, None, None, None
@@ -251,7 +280,8 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, r, t, keep):
         loss, per_row, stats, ctx.d = _distill(logits.device, logits, r, t, keep, True)
-        ctx.r, ctx.t, ctx.keep = r, t, keep
+        _keep(ctx, logits, r, keep)
+        ctx.t, ctx.capture = t, _capture(logits.device)
         ctx.save_for_backward(logits, stats)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(per_row)
@@ -262,10 +292,14 @@ class _Distill(torch.autograd.Function):
         if g is None:
             return None, None, None, None
         logits, stats = ctx.saved_tensors
+        r, moved = _kept(ctx, logits)
         # the forward pass has written the gradient for g = 1 (a loss that is not scaled further): any other g forms it
-        # again from the logits, on the device; a second backward pass has a gradient of its own
+        # again from the logits, on the device; a second backward pass has a gradient of its own, and so has one that is
+        # recorded without its forward pass, which may be replayed more often
         d, ctx.d = ctx.d, None
-        d = _distill_backward(logits.device, logits, ctx.r, ctx.t, g, stats, d)
+        if ctx.capture != _capture(logits.device):
+            d = None
+        d = _distill_backward(logits.device, logits, r, ctx.t, g, stats, d)
         return _Once.apply(d, logits) if torch.is_grad_enabled() else d, None, None, None
 
 
@@ -274,7 +308,7 @@ def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None
 
         KL_row = sum_j p_j (log p_j - log q_{i_j}),   p = softmax(top_logits / T),   q = softmax(logits / T)
 
-    Returns (loss, per_row): loss = sum over rows of weight * KL_row (weight 1 unless given; give 1 / rows for a mean,
+    Returns (loss, per_row): loss = sum over rows of weight * KL_row (a tensor or a number, 1 unless given; 1 / rows for a mean,
     T^2 for the customary scale, 0 for the rows to leave out: those are not read), differentiable with respect to the
     logits, and KL_row itself, float32, without gradient.  The gradient is formed in the pass that forms the loss; an
     upstream gradient other than 1 costs a second pass.
@@ -291,6 +325,8 @@ def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None
     if top_logits.dtype not in _DTYPES:
         raise TypeError(f"top_logits of type {top_logits.dtype}: float32, bfloat16 or float16")
     _integers(top_index, "top_index")
+    if isinstance(weight, (int, float)):
+        weight = torch.full((), float(weight), device=logits.device)
     if torch.is_grad_enabled() and (top_logits.requires_grad or (weight is not None and weight.requires_grad)):
         raise ValueError("the teacher's logits and the weights have no gradient: detach them")
     k = top_logits.shape[-1]

@@ -16,7 +16,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kClampD = -256.f;        // 2^d is 0 below: keeps 0 * (-inf) out of the entropy sum
+constexpr float kClampD = -256.f;        // 2^d (and e^d) is 0 below: keeps 0 * (-inf) out of sums and products
 constexpr float kNearCertain = 0.0625f;  // below this r the largest category's thread sums its other terms again
 constexpr int kMaxTop = DMV_CAT_MAX_TOP;
 constexpr int kMaxTeacher = DMV_CAT_MAX_TEACHER;
@@ -232,6 +232,8 @@ struct Fwd {
   int parts;     // workgroups per row; > 1: partial results go to ws
   f32x4* part;   // [rows][parts] (m, r, u, -)
   uint2* part_top;  // [rows][parts][top] (key, index), in order; key 0 past the end
+  const float* weight;  // nullable, for distillation: rows of weight 0 are not read
+  int64_t w_period;
 };
 
 struct Bwd {
@@ -335,10 +337,10 @@ struct RowGrad {
   __device__ __forceinline__ float dense(float x) const {
     const float y = x - m;
     const float q = exp2_hw(y * kLog2e) * inv_s;
-    return -q * (S + gh * (fmaxf(y - logs, -1e30f) + H));
+    return -q * (S + gh * (fmaxf(y - logs, kClampD) + H));
   }
   __device__ __forceinline__ float at(float x, float a) const {
-    const float lq = fmaxf(x - m - logs, -1e30f);
+    const float lq = fmaxf(x - m - logs, kClampD);
     const float q = exp2_hw(lq * kLog2e);
     return -a * expm1f(lq) - (S - a) * q - gh * q * (lq + H);
   }
@@ -849,108 +851,108 @@ __global__ void __launch_bounds__(NT) k_cat_distill_small(Dist a) {
   const int lane = threadIdx.x & (L - 1), V = a.r.V, K = a.t.k, g = threadIdx.x / L;
   double part = 0.0;
   for (int row = blockIdx.x * NG + g; row < (int)a.r.rows; row += NG) {
-  const float w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
-  float kl = 0.f;
-  if (w != 0.f) {
-    const char* p = a.r.x + row * a.r.ld * ES;
-    SmallRow<DT, VEC, L, SL> x;
-    x.load(p, V, lane);
-    const int n = row_size(a.r, row);
-    Entry* own = entries + g * K;
-    const int64_t t0 = wrap(row, a.t.t_period, a.r.rows) * K;
-    float tm = -INFINITY;
-    uint32_t flags = 0;                 // 1: an entry counts, 2: one that cannot be
-    for (int j = lane; j < K; j += L) {
-      const int64_t i = a.t.idx[t0 + j];
-      const float t = teacher_logit(a.t, t0 + j);
-      const bool counts = entry_counts(t, i), bad = counts && (i >= n || !(t < INFINITY));
-      flags |= (counts ? 1u : 0u) | (bad ? 2u : 0u);
-      if (counts) tm = fmaxf(tm, t);
-      own[j] = Entry{t, counts && !bad ? Elem<DT>::load(p, i) : 0.f, counts && !bad ? (int)i : -1};
-    }
-    tm = gmax<L>(tm);
-    flags = gmax_u<L>(flags);
-    const bool any = flags != 0u, bad = flags >= 2u;
-    float m, r, u, kept[E];
-    x.count_once(V, n, lane);
-    small_stats<false, true>(x, a.t.c, m, r, u, kept);      // (twice the registers of the packed row, but no second exp2)
-    const bool empty = m == -INFINITY && !(r != r);
-    const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
-    const bool live = any && !empty;
-    if (live && !bad) {
-      float s = 0.f, held = 0.f;
-      for (int j = lane; j < K; j += L)
-        if (own[j].i >= 0) {
-          if (own[j].t == tm) held += 1.f;
-          else s += exp2_hw((own[j].t - tm) * a.t.c);
-        }
-      const float t_logs = log1p_row(rsum<L>(s) + (rsum<L>(held) - 1.f));
-      for (int j = lane; j < K; j += L)
-        if (own[j].i >= 0) {
-          const float lp = (own[j].t - tm) * a.t.inv_T - t_logs, q = exp_hw(lp), lq = (own[j].x - m) * a.t.inv_T - logs;
-          if (q > 0.f) kl += q * (lp - lq);
-          own[j].t = lp;
-          own[j].x = lq;
-        }
-      kl = rsum<L>(kl);
-    }
-    if (any && empty) kl = INFINITY;
-    if (bad) kl = NAN;
-    if (lane == 0) part += (double)w * (double)kl;
-    if (a.d) {
-      char* out = (char*)a.d + row * a.ld_d * ES;
-      const float scale = bad ? NAN : gs * w * a.t.inv_T, f = scale * inv_s;
-      if (!live) small_zeros<DT, VEC, L>(out, V, lane);
-#pragma unroll
-      for (int j = 0; j < SL; ++j) {
-        const int fst = (lane + L * j) * VEC;
-        if (fst >= V || !live) continue;
-        float v[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = f * kept[j * VEC + e];     // (what does not count: 0)
-        if (fst + VEC <= V) slot_store<DT, VEC>(out, fst, v);
-        else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (V - VEC + e >= fst) Elem<DT>::store(out, V - VEC + e, v[e]);
-        }
+    const float w = a.t.weight ? a.t.weight[wrap(row, a.t.w_period, a.r.rows)] : 1.f;
+    float kl = 0.f;
+    if (w != 0.f) {
+      const char* p = a.r.x + row * a.r.ld * ES;
+      SmallRow<DT, VEC, L, SL> x;
+      x.load(p, V, lane);
+      const int n = row_size(a.r, row);
+      Entry* own = entries + g * K;
+      const int64_t t0 = wrap(row, a.t.t_period, a.r.rows) * K;
+      float tm = -INFINITY;
+      uint32_t flags = 0;                 // 1: an entry counts, 2: one that cannot be
+      for (int j = lane; j < K; j += L) {
+        const int64_t i = a.t.idx[t0 + j];
+        const float t = teacher_logit(a.t, t0 + j);
+        const bool counts = entry_counts(t, i), bad = counts && (i >= n || !(t < INFINITY));
+        flags |= (counts ? 1u : 0u) | (bad ? 2u : 0u);
+        if (counts) tm = fmaxf(tm, t);
+        own[j] = Entry{t, counts && !bad ? Elem<DT>::load(p, i) : 0.f, counts && !bad ? (int)i : -1};
       }
+      tm = gmax<L>(tm);
+      flags = gmax_u<L>(flags);
+      const bool any = flags != 0u, bad = flags >= 2u;
+      float m, r, u, kept[E];
+      x.count_once(V, n, lane);
+      small_stats<false, true>(x, a.t.c, m, r, u, kept);      // (twice the registers of the packed row, but no second exp2)
+      const bool empty = m == -INFINITY && !(r != r);
+      const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
+      const bool live = any && !empty;
       if (live && !bad) {
-        // A category given more than once has all its entries' probability in each of them.  Whether there is one is told
-        // by a bit per category.
-        bool twice = K <= kFewEntries;
-        if (!twice) {
-          for (int q = lane; q < WORDS; q += L) given[g][q] = 0u;
-          wave_sync();
-          for (int j = lane; j < K; j += L)
-            if (own[j].i >= 0) {
-              const uint32_t bit = 1u << (own[j].i & 31);
-              twice = twice || (atomicOr(&given[g][own[j].i >> 5], bit) & bit) != 0u;
-            }
-          twice = gmax_u<L>(twice ? 1u : 0u) != 0u;
-        }
-        // the dense part before the teacher's categories are written again: stores of one wavefront stay in order
-        wave_sync();
-        for (int j = lane; j < K; j += L) {
-          const Entry e = own[j];
-          if (e.i < 0) continue;
-          float lp = e.t;
-          if (twice) {
-            int same = 0;
-            float sum = 0.f;
-            for (int h = 0; h < K; ++h)
-              if (own[h].i == e.i) sum += exp_hw(own[h].t), ++same;
-            if (same > 1) lp = logf(sum);
+        float s = 0.f, held = 0.f;
+        for (int j = lane; j < K; j += L)
+          if (own[j].i >= 0) {
+            if (own[j].t == tm) held += 1.f;
+            else s += exp2_hw((own[j].t - tm) * a.t.c);
           }
-          Elem<DT>::store(out, e.i, scale * q_minus_p(e.x, lp));
+        const float t_logs = log1p_row(rsum<L>(s) + (rsum<L>(held) - 1.f));
+        for (int j = lane; j < K; j += L)
+          if (own[j].i >= 0) {
+            const float lp = (own[j].t - tm) * a.t.inv_T - t_logs, q = exp_hw(lp), lq = (own[j].x - m) * a.t.inv_T - logs;
+            if (q > 0.f) kl += q * (lp - lq);
+            own[j].t = lp;
+            own[j].x = lq;
+          }
+        kl = rsum<L>(kl);
+      }
+      if (any && empty) kl = INFINITY;
+      if (bad) kl = NAN;
+      if (lane == 0) part += (double)w * (double)kl;
+      if (a.d) {
+        char* out = (char*)a.d + row * a.ld_d * ES;
+        const float scale = bad ? NAN : gs * w * a.t.inv_T, f = scale * inv_s;
+        if (!live) small_zeros<DT, VEC, L>(out, V, lane);
+  #pragma unroll
+        for (int j = 0; j < SL; ++j) {
+          const int fst = (lane + L * j) * VEC;
+          if (fst >= V || !live) continue;
+          float v[VEC];
+  #pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = f * kept[j * VEC + e];     // (what does not count: 0)
+          if (fst + VEC <= V) slot_store<DT, VEC>(out, fst, v);
+          else {
+  #pragma unroll
+            for (int e = 0; e < VEC; ++e)
+              if (V - VEC + e >= fst) Elem<DT>::store(out, V - VEC + e, v[e]);
+          }
+        }
+        if (live && !bad) {
+          // A category given more than once has all its entries' probability in each of them.  Whether there is one is told
+          // by a bit per category.
+          bool twice = K <= kFewEntries;
+          if (!twice) {
+            for (int q = lane; q < WORDS; q += L) given[g][q] = 0u;
+            wave_sync();
+            for (int j = lane; j < K; j += L)
+              if (own[j].i >= 0) {
+                const uint32_t bit = 1u << (own[j].i & 31);
+                twice = twice || (atomicOr(&given[g][own[j].i >> 5], bit) & bit) != 0u;
+              }
+            twice = gmax_u<L>(twice ? 1u : 0u) != 0u;
+          }
+          // the dense part before the teacher's categories are written again: stores of one wavefront stay in order
+          wave_sync();
+          for (int j = lane; j < K; j += L) {
+            const Entry e = own[j];
+            if (e.i < 0) continue;
+            float lp = e.t;
+            if (twice) {
+              int same = 0;
+              float sum = 0.f;
+              for (int h = 0; h < K; ++h)
+                if (own[h].i == e.i) sum += exp_hw(own[h].t), ++same;
+              if (same > 1) lp = logf(sum);
+            }
+            Elem<DT>::store(out, e.i, scale * q_minus_p(e.x, lp));
+          }
         }
       }
+    } else if (a.d) {
+      small_zeros<DT, VEC, L>((char*)a.d + row * a.ld_d * ES, V, lane);
     }
-  } else if (a.d) {
-    small_zeros<DT, VEC, L>((char*)a.d + row * a.ld_d * ES, V, lane);
-  }
-  if (lane == 0 && a.per_row) a.per_row[(uint32_t)row] = kl;
-  if (!LONE) break;
+    if (lane == 0 && a.per_row) a.per_row[(uint32_t)row] = kl;
+    if (!LONE) break;
   }
   // the workgroup's share of the loss, in a fixed order
 #pragma unroll
@@ -1150,10 +1152,10 @@ __device__ __forceinline__ void rank_candidates(cand_t* cand, int have, int k, E
 // The selection's result goes through `emit(rank, key, index)`.
 //
 // Every thread knows the largest value of each of its slot groups.  tau, at most the k-th largest of the largest values of
-// 256 threads (or sets of threads), is a lower bound of the k-th largest element, so only groups whose largest value reaches tau hold
-// any of the k: these are listed, read again with a slot per thread, and the elements that reach tau - little more than k
-// in an ordinary row - are ranked by counting.  Rows with more candidates than fit (many equal values) take the
-// ordered scan below, and in the worst case one pass over the listed groups per rank.
+// 256 threads (or sets of threads), is a lower bound of the k-th largest element, so only groups whose largest value
+// reaches tau hold any of the k: these are listed, read again with a slot per thread, and the elements that reach tau -
+// little more than k in an ordinary row - are ranked by counting.  Rows with more candidates than fit (many equal values)
+// take the ordered scan below, and in the worst case one pass over the listed groups per rank.
 template <int DT, int VEC, int NT, typename Emit>
 __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& span, int s0, int s1, int gsz, int k, float m, float tmax,
                           Emit emit) {
@@ -1352,6 +1354,7 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
     if (tid == 0 && part == 0 && a.log_prob) a.log_prob[row] = 0.f;
     return;
   }
+  if (!ENT && !TOP && a.weight && a.weight[wrap(row, a.w_period, a.r.rows)] == 0.f) return;
   const int n = row_size(a.r, row);
   const char* p = a.r.x + row * a.r.ld * ES;
   const Span<VEC> span(p, ES, a.r.V, n);
@@ -1631,8 +1634,8 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_bwd_chunk(Bwd a) {
 }
 
 
-// The teacher's distribution over one row by a workgroup, entry j on thread j (the launch has k <= NT): p and log p of this thread's entry
-// (p = 0 where it does not count), its index (-1), and what holds for the row.
+// The teacher's distribution over one row by a workgroup, entry j on thread j (the launch has k <= NT): p and log p of this
+// thread's entry (p = 0 where it does not count), its index (-1), and what holds for the row.
 struct TeacherEntry {
   float p, lp;
   int i;
@@ -1933,8 +1936,9 @@ int check_rows(const DmvCatRows* r) {
   if (r->rows == 0) return DMV_OK;
   if (!r->logits || ((uintptr_t)r->logits % elem_size(r->dtype)) != 0) return DMV_E_BADARG;
   if ((r->X && r->x_period < 1) || (r->M && r->m_period < 1) || (r->sizes && r->size_period < 1)) return DMV_E_BADARG;
-  // row numbers of short rows and threads of a launch in 32 bits, slot numbers in 32 bits with room for a chunk
-  if (r->rows >= (int64_t)1 << 26 || r->V > 0x7fffffff - (1 << 20)) return DMV_E_UNSUPPORTED;
+  // row numbers of short rows and threads of a launch (64 a row, whole workgroups) in 32 bits, slot numbers in 32 bits with
+  // room for a chunk
+  if (r->rows >= ((int64_t)1 << 26) - 4 || r->V > 0x7fffffff - (1 << 20)) return DMV_E_UNSUPPORTED;
   return DMV_OK;
 }
 bool fits_grid(int64_t groups, int threads) { return groups * threads < (int64_t)1 << 32; }
@@ -2065,7 +2069,7 @@ extern "C" int dmv_cat_log_prob(const DmvCatRows* r, float* log_prob, float* ent
   if (r->rows == 0) return DMV_OK;
   if ((log_prob && !r->X) || (!log_prob && !entropy && !top) || (top && (!top_log_prob || !top_index))) return DMV_E_BADARG;
   if (((uintptr_t)stats & 15) != 0 || ((uintptr_t)ws & 15) != 0) return DMV_E_BADARG;
-  Fwd a{rows_of(r), log_prob, entropy, top, top_log_prob, top_index, (f32x4*)stats, kLog2e, 1, nullptr, nullptr};
+  Fwd a{rows_of(r), log_prob, entropy, top, top_log_prob, top_index, (f32x4*)stats, kLog2e, 1, nullptr, nullptr, nullptr, 0};
   hipStream_t st = (hipStream_t)stream;
   if (r->V <= kSmallMax) {
     by_type(r->dtype, [&](auto dt) {
@@ -2142,12 +2146,14 @@ static int check_teacher(const DmvCatRows* r, const DmvCatTeacher* t) {
 static Dist dist_of(const DmvCatRows* r, const DmvCatTeacher* t) {
   Dist a{};
   a.r = rows_of(r);
+  a.r.X = nullptr, a.r.M = nullptr;      // which rows count is said by the weights
   a.t = Teacher{t->logits, t->index, t->weight, t->period, t->w_period, t->k, t->dtype, kLog2e / t->temperature, 1.f / t->temperature};
   a.chunks = a.parts = 1;
   return a;
 }
-// A small launch: one workgroup does all rows in two rounds at most, and the loss.  (64 x 1000 float32, two rounds: 15.6 us on
-// the GPU instead of 6.1 + 1.6, but a launch less of the host's 90 us a step; each further round takes 6 us more.)
+// A small launch: one workgroup does all rows in two rounds at most, and the loss.  A launch less for the host: 16 x 25
+// float32 a step of 84 us instead of 93, 64 x 1000 84 instead of 93, each step waited for 100 instead of 108.  On the GPU
+// alone, as in a replayed graph, 5.6 us instead of 6.9, and 15.3 instead of 7.6: a third round would lose what it saves.
 template <typename T>
 bool lone_group(int64_t rows, int k) {
   return rows <= 2 * (kLoneThreads / T::L) && (size_t)(kLoneThreads / T::L) * k * sizeof(Entry) <= 48 * 1024;
@@ -2202,7 +2208,8 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
         typedef decltype(tile) T;
         if (lone_group<T>(r->rows, t->k)) {
           a.loss = loss;
-          k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kLoneThreads><<<1, kLoneThreads, small_lds<T>(t->k) * (kLoneThreads / kSmallThreads), st>>>(a);
+          const size_t lds = small_lds<T>(t->k) * (kLoneThreads / kSmallThreads);
+          k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kLoneThreads><<<1, kLoneThreads, lds, st>>>(a);
         } else {
           k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kSmallThreads><<<(unsigned)n_loss, kSmallThreads, small_lds<T>(t->k), st>>>(a);
         }
@@ -2218,7 +2225,7 @@ extern "C" int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, floa
     if (!a.stats) a.stats = own;
     a.part = own + r->rows;
     a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
-    Fwd f{a.r, nullptr, nullptr, 0, nullptr, nullptr, nullptr, a.t.c, a.parts, a.part, nullptr};
+    Fwd f{a.r, nullptr, nullptr, 0, nullptr, nullptr, nullptr, a.t.c, a.parts, a.part, nullptr, a.t.weight, a.t.w_period};
     const int64_t items = r->rows * a.chunks;
     by_type(r->dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
@@ -2254,7 +2261,8 @@ extern "C" int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher
     if (r->V <= kSmallMax) {
       teacher_tile<DT>(r->V, t->k, [&](auto tile) {
         typedef decltype(tile) T;
-        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kSmallThreads><<<(unsigned)T::groups(r->rows), kSmallThreads, small_lds<T>(t->k), st>>>(a);
+        const dim3 grid((unsigned)T::groups(r->rows));
+        k_cat_distill_small<T::DT, T::VEC, T::L, T::SL, kSmallThreads><<<grid, kSmallThreads, small_lds<T>(t->k), st>>>(a);
       });
     } else {
       a.chunks = dmv_ceil_div(row_slots(r->V, r->dtype), kChunkSlots);
@@ -2264,4 +2272,14 @@ extern "C" int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher
   });
   DMV_HIP_CHECK_LAUNCH();
   return DMV_OK;
+}
+
+extern "C" uint64_t dmv_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
 }

@@ -521,7 +521,7 @@ int dmv_grid_divergences(int32_t gen_dist, int32_t D, int32_t Zd, int64_t Nz, co
  * A row without any category of non-zero probability (size 0, or all logits -inf) has entropy 0, log-probability -inf,
  * no alternatives and a zero gradient.  NaN or +inf among a row's logits makes its outputs NaN (alternatives -1); a given
  * category outside the row's, where it is seen, makes that row's log-probability and gradient NaN.
- * Limits (DMV_E_UNSUPPORTED): fewer than 2^26 rows (2^24 where V > DMV_CAT_SHORT_ROW), V below 2^31 - 2^20. */
+ * Limits (DMV_E_UNSUPPORTED): fewer than 2^26 - 4 rows (2^24 where V > DMV_CAT_SHORT_ROW), V below 2^31 - 2^20. */
 enum { DMV_F32 = 0, DMV_BF16 = 1, DMV_F16 = 2 };
 #define DMV_CAT_MAX_TOP 64
 #define DMV_CAT_MAX_TEACHER 256
@@ -557,7 +557,7 @@ int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats, const flo
  * r % period (an entry with a negative index or a logit of -inf is empty; a category given twice counts twice) and q =
  * softmax(row / T) over all of the row's categories,
  *   per_row[r] = KL(p || q) = sum_j p_j (log p_j - log q_index[j]),   loss = sum_r weight[r % w_period] per_row[r]
- * (weight NULL: 1).  Rows of weight 0 are not read and have per_row 0; rows without entries have 0.  d_logits (nullable)
+ * (weight NULL: 1; X and M of the rows are not looked at).  Rows of weight 0 are not read and have per_row 0; rows without entries have 0.  d_logits (nullable)
  * receives the gradient of loss: weight / T (q - p).  An index at or past the row's size, or a logit of NaN or +inf,
  * makes the row's loss and gradient NaN; categories of probability 0 under q with p > 0 make the loss inf.  The sum of
  * the loss has a fixed order and is held in 64 bits.
@@ -580,6 +580,10 @@ int dmv_cat_distill(const DmvCatRows* r, const DmvCatTeacher* t, float* per_row,
  * device, if *gscale is 1: d_logits already holds what dmv_cat_distill wrote. */
 int dmv_cat_distill_backward(const DmvCatRows* r, const DmvCatTeacher* t, const float* gscale, int32_t unless_one,
                              const float* stats, void* d_logits, int64_t ld_d, void* stream);
+/* Number of the graph capture that `stream` is in, 0 outside any.  A gradient that dmv_cat_distill left in a buffer may be
+ * handed on (unless_one) by a backward call of the same capture only: a graph with the backward call alone can be replayed
+ * more than once for one replay of the forward call's. */
+uint64_t dmv_capture_id(void* stream);
 
 /* Optimiser step (vgiwae/models/vae.py:349-390: Adam / AMSGrad with one parameter group per network, preceded by
  * clip_grad_norm_ over all parameters; shared/mvb2_manual_optimisation.py:9-11).  One call =

@@ -165,3 +165,23 @@ def test_distill_entry_refuses_outputs_and_workspace():
     big = C.byref(_rows(V=5000, ld=5000))
     assert lib.dmv_cat_distill_backward(big, t, FAKE, 0, None, FAKE, 5000, None) == BAD      # long rows need their statistics
     assert lib.dmv_cat_distill_backward(r, t, None, 0, FAKE, FAKE, 8, None) == BAD
+
+
+def test_more_categories_than_an_index_holds():
+    x = torch.empty(1, 2 ** 31, dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="categories"):
+        dmv.categorical_log_prob(x, entropy=True)
+    with pytest.raises(ValueError, match="categories"):
+        dmv.distill_top_logits(x, torch.zeros(1, 2), torch.zeros(1, 2, dtype=torch.long))
+
+
+def test_entries_refuse_rows_beyond_the_grid_of_the_widest_tile():
+    """64 lanes a row: 2^26 - 4 rows would take 2^32 threads"""
+    r = C.byref(_rows(rows=(1 << 26) - 4, V=2048, ld=2048))
+    assert L.lib().dmv_cat_log_prob(r, FAKE, None, 0, None, None, None, None, 0, None) == UNSUPPORTED
+    assert L.lib().dmv_cat_distill(r, C.byref(_teacher()), None, FAKE, None, None, 0, FAKE, 1 << 40, None) == UNSUPPORTED
+
+
+def test_a_number_as_weight_is_an_argument():
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        dmv.distill_top_logits(_logits(4, 7), torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), weight=0.25)

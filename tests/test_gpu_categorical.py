@@ -788,3 +788,142 @@ def test_offsets_past_32_bits():
     close(per_row[-3:], kl, tol, "kl")
     close(dx[-3:], g, tol_g + narrow(g, torch.bfloat16), "gradient")
     assert not bool(dx[:-3].any())
+
+
+# ------------------------------------------------------------------------------------------ what a backward pass holds
+def _losses(V, n=4):
+    x = make((n, V), torch.float32)
+    X = ints(V, (n,))
+    t, idx = teacher_of(x, 3)
+    return x, [lambda z: dmv.categorical_log_prob(z, X, entropy=True).log_prob.sum(), lambda z: dmv.distill_top_logits(z, t, idx)[0] * 2.0]
+
+
+@pytest.mark.parametrize("V", [40, 5000, 90000])
+def test_saved_logits_come_back_from_elsewhere(V):
+    """saved tensors kept on the host, or computed again: the first copy's memory is somebody else's by then"""
+    from torch.utils.checkpoint import checkpoint
+    x, losses = _losses(V)
+    for f in losses:
+        z = x.clone().requires_grad_()
+        (want,) = torch.autograd.grad(f(1.0 * z), z)
+        for rows in (lambda y: y, lambda y: torch.cat([y, y], -1)[:, :V], lambda y: (1.0 * y.t()).t()):     # a pitch; a copy
+            with torch.autograd.graph.save_on_cpu():
+                loss = f(rows(1.0 * z))
+            others = [torch.full((4, V), 7.0, device="cuda") for _ in range(8)]
+            (got,) = torch.autograd.grad(loss, z)
+            assert torch.equal(got, want)
+            loss = checkpoint(lambda z: f(rows(1.0 * z)), z, use_reentrant=False)
+            others += [torch.full((4, V), 7.0, device="cuda") for _ in range(8)]
+            (got,) = torch.autograd.grad(loss, z)
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("V", [40, 5000])
+def test_arguments_modified_before_the_backward_pass(V):
+    n = 4
+    x = make((n, V), torch.float32)
+
+    def refused(loss, z, t):
+        t.add_(1) if t.dtype != torch.bool else t.logical_not_()
+        with pytest.raises(RuntimeError, match="modified in place"):
+            torch.autograd.grad(loss, z)
+
+    for name in ("X", "M", "sizes"):
+        a = dict(X=ints(V - 1, (n,)), M=rand((n,)) < 0.5, sizes=torch.full((n,), V - 1, dtype=torch.int32, device="cuda"))
+        z = x.clone().requires_grad_()
+        refused(dmv.categorical_log_prob(z, **a).log_prob.sum(), z, a[name])
+    for name in ("top_logits", "top_index", "weight", "sizes"):
+        t, idx = teacher_of(x[:, :V - 1], 3)
+        a = dict(top_logits=t, top_index=idx, weight=rand((n,)), sizes=torch.full((n,), V - 1, dtype=torch.int32, device="cuda"))
+        z = x.clone().requires_grad_()
+        refused(dmv.distill_top_logits(z, **a)[0], z, a[name])
+
+
+@pytest.mark.parametrize("V", [40, 5000])
+def test_a_teacher_in_inference_mode(V):
+    x = make((4, V), torch.float32, seed=2)
+    with torch.inference_mode():
+        a = dmv.categorical_log_prob(make((4, V), torch.float32, seed=1), top=5)
+    check_distill(x, a.top_log_prob.clone(), a.top_index.clone())
+    z = x.clone().requires_grad_()
+    (got,) = torch.autograd.grad(dmv.distill_top_logits(z, a.top_log_prob, a.top_index)[0], z)
+    (want,) = torch.autograd.grad(dmv.distill_top_logits(z, a.top_log_prob.clone(), a.top_index.clone())[0], z)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("V", [40, 5000, 90000])
+def test_forward_and_backward_in_graphs_of_their_own(V):
+    """the backward pass replayed twice for one forward pass, with another upstream gradient each time"""
+    x = make((4, V), torch.float32)
+    t, idx = teacher_of(x, 3)
+    z, u = x.clone().requires_grad_(), torch.ones((), device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss, _ = dmv.distill_top_logits(z, t, idx)
+        want = torch.autograd.grad(loss, z)[0].clone()
+    del loss
+    torch.cuda.synchronize()
+    fwd, bwd = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(fwd, stream=s):
+        loss, _ = dmv.distill_top_logits(z, t, idx)
+    with torch.cuda.graph(bwd, stream=s):
+        (g,) = torch.autograd.grad(loss, z, u)
+    for _ in range(2):
+        fwd.replay()
+        for up in (2.0, 1.0, -4.0, 1.0):
+            u.fill_(up)
+            bwd.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(g, want if up == 1.0 else up * want), up      # (powers of two)
+
+
+# ------------------------------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("V", [300, 3000])
+def test_sizes_of_every_integer_type(V):
+    x = make((3, V), torch.float32)
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64):
+        sizes = torch.tensor([3, 100, 127], dtype=dtype, device="cuda")
+        check_log_prob(x, sizes=sizes, entropy=True)
+
+
+@pytest.mark.parametrize("V", [40, 3000])
+def test_weight_as_a_number(V):
+    x = make((4, V), torch.float32)
+    t, idx = teacher_of(x, 3)
+    z = x.clone().requires_grad_()
+    a = dmv.distill_top_logits(z, t, idx, weight=0.25)
+    b = dmv.distill_top_logits(z, t, idx, weight=torch.full((4,), 0.25, device="cuda"))
+    assert torch.equal(a[0], b[0]) and torch.equal(*(torch.autograd.grad(o[0], z)[0] for o in (a, b)))
+
+
+@pytest.mark.parametrize("V", [40, 5000])
+def test_large_upstream_gradient_of_the_entropy_leaves_masked_places(V):
+    x = make((3, V), torch.float32)
+    x[:, ::2] = -math.inf
+    z = x.requires_grad_()
+    (dx,) = torch.autograd.grad(dmv.categorical_log_prob(z, entropy=True).entropy.sum() * 2.0 ** 80, z)
+    assert bool((dx[:, ::2] == 0).all()) and bool(torch.isfinite(dx).all())
+
+
+@pytest.mark.parametrize("V", [40, 5000, 90000])
+def test_distillation_looks_at_weights_and_not_at_the_rows_mask(V):
+    """rows of weight 0 hold NaN; the C entry given the rows' X and M as well"""
+    import ctypes as C
+    from demiss_vae_amd import _lib as L
+    x = make((5, V), torch.float32)
+    t, idx = teacher_of(x, 3)
+    w = torch.tensor([1.0, 0.0, 2.0, 0.0, 1.0], device="cuda")
+    loss, per_row = dmv.distill_top_logits(x, t, idx, weight=w)
+    x[w == 0] = math.nan
+    again = dmv.distill_top_logits(x, t, idx, weight=w)
+    assert torch.equal(again[0], loss) and torch.equal(again[1], per_row)
+    X, M = ints(V, (5,)), torch.zeros(5, dtype=torch.bool, device="cuda")
+    r = L.DmvCatRows(logits=x.data_ptr(), ld=V, rows=5, V=V, dtype=0, X=X.data_ptr(), x_period=5, M=M.data_ptr(), m_period=5)
+    tc = L.DmvCatTeacher(logits=t.data_ptr(), index=idx.data_ptr(), period=5, k=3, dtype=0, weight=w.data_ptr(), w_period=5, temperature=1.0)
+    n = L.lib().dmv_cat_distill_ws_bytes(C.byref(r), 3)
+    ws = torch.empty(n // 4 + 4, device="cuda")
+    out, rows = torch.empty((), device="cuda"), torch.empty(5, device="cuda")
+    L.check(L.lib().dmv_cat_distill(C.byref(r), C.byref(tc), rows.data_ptr(), out.data_ptr(), None, None, 0, ws.data_ptr(), n,
+                                    torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out, loss) and torch.equal(rows, per_row)
