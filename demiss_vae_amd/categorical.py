@@ -124,22 +124,25 @@ def _set_logits(r, logits, keep):
 def _keep(ctx, logits, r, keep):
     """What a backward pass needs of a call's arguments.  Its arrays are held here, and their versions, because pointers to
     them are: saved tensors may come back from elsewhere, and may not have been made for saving (a teacher's, say)."""
-    ctx.r, ctx.keep, ctx.versions = r, keep, _versions(keep)
-    ctx.in_place = r.logits == logits.data_ptr()
+    ctx.kept = r, keep, _versions(keep), r.logits == logits.data_ptr()
 
 
 def _versions(keep):
-    return [0 if t.is_inference() else t._version for t in keep]
+    try:
+        return [t._version for t in keep]
+    except RuntimeError:                    # one made in inference mode, which counts no versions
+        return [0 if t.is_inference() else t._version for t in keep]
 
 
 def _kept(ctx, logits):
     """The call's rows for its backward pass, with the saved logits where they are now; and what has to stay alive."""
-    if _versions(ctx.keep) != ctx.versions:
+    r, keep, versions, in_place = ctx.kept
+    if _versions(keep) != versions:
         raise RuntimeError("a tensor that the gradient of a categorical operator needs (X, M, sizes, weight or the teacher's) "
                            "was modified in place after the forward call")
-    if not ctx.in_place or ctx.r.logits == logits.data_ptr():
-        return ctx.r, None
-    r, moved = L.DmvCatRows.from_buffer_copy(ctx.r), []
+    if not in_place or r.logits == logits.data_ptr():
+        return r, None
+    r, moved = L.DmvCatRows.from_buffer_copy(r), []
     _set_logits(r, logits, moved)
     return r, moved
 
@@ -152,8 +155,9 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _capture(device):
-    return L.lib().dmv_capture_id(_stream(device))
+def _capture(stream):
+    """The graph capture that the current stream is in, 0 outside any."""
+    return L.lib().dmv_capture_id(stream) if torch._C._cuda_isCurrentStreamCapturing() else 0
 
 
 def _on_device(f):
@@ -261,27 +265,30 @@ def _distill(dev, logits, r, t, keep, training):
     n_stats = 4 * r.rows if training and r.V > L.CAT_SHORT_ROW else 0
     n_ws = lib.dmv_cat_distill_ws_bytes(C.byref(r), t.k)
     stats = torch.empty(n_stats + n_ws // 4, dtype=torch.float32, device=dev) if n_stats or n_ws else None      # as in _log_prob
-    at = L.addr(stats)
+    at, stream = L.addr(stats), _stream(dev)
     L.check(lib.dmv_cat_distill(C.byref(r), C.byref(t), per_row.data_ptr(), loss.data_ptr(), at if n_stats else None, L.addr(d), r.V,
-                                at + 4 * n_stats if n_ws else None, n_ws, _stream(dev)))
-    return loss, per_row, stats, d
+                                at + 4 * n_stats if n_ws else None, n_ws, stream))
+    return loss, per_row, stats, (d, _capture(stream)) if training else None
 
 
 @_on_device
-def _distill_backward(dev, logits, r, t, g, stats, d):
-    unless_one = d is not None
-    if d is None:
-        d = _like(logits)
-    L.check(L.lib().dmv_cat_distill_backward(C.byref(r), C.byref(t), L.addr(g), unless_one, L.addr(stats), L.addr(d), r.V, _stream(dev)))
+def _distill_backward(dev, logits, r, t, g, stats, formed):
+    # the forward pass has written the gradient for g = 1 (a loss that is not scaled further): any other g forms it again
+    # from the logits, on the device; a second backward pass has a gradient of its own, and so has one that is recorded
+    # without its forward pass, which may be replayed more often
+    stream = _stream(dev)
+    unless_one = formed is not None and formed[1] == _capture(stream)
+    d = formed[0] if unless_one else _like(logits)
+    L.check(L.lib().dmv_cat_distill_backward(C.byref(r), C.byref(t), L.addr(g), unless_one, L.addr(stats), L.addr(d), r.V, stream))
     return d
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, r, t, keep):
-        loss, per_row, stats, ctx.d = _distill(logits.device, logits, r, t, keep, True)
+        loss, per_row, stats, ctx.formed = _distill(logits.device, logits, r, t, keep, True)
         _keep(ctx, logits, r, keep)
-        ctx.t, ctx.capture = t, _capture(logits.device)
+        ctx.t = t
         ctx.save_for_backward(logits, stats)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(per_row)
@@ -293,13 +300,8 @@ class _Distill(torch.autograd.Function):
             return None, None, None, None
         logits, stats = ctx.saved_tensors
         r, moved = _kept(ctx, logits)
-        # the forward pass has written the gradient for g = 1 (a loss that is not scaled further): any other g forms it
-        # again from the logits, on the device; a second backward pass has a gradient of its own, and so has one that is
-        # recorded without its forward pass, which may be replayed more often
-        d, ctx.d = ctx.d, None
-        if ctx.capture != _capture(logits.device):
-            d = None
-        d = _distill_backward(logits.device, logits, r, ctx.t, g, stats, d)
+        formed, ctx.formed = ctx.formed, None
+        d = _distill_backward(logits.device, logits, r, ctx.t, g, stats, formed)
         return _Once.apply(d, logits) if torch.is_grad_enabled() else d, None, None, None
 
 
