@@ -673,7 +673,7 @@ __device__ __forceinline__ void small_sorted(const float* o, int V, int lane, in
   for (int j = E * L + lane; j < k; j += L) emit(j, -INFINITY, -1);
 }
 
-// Short rows, forward.  Bound by the vector units and not by memory: of 706 instructions that a wavefront takes for eight rows
+// Short rows, forward.  Bound by the vector units (92 % busy) and not by memory: of 743 instructions that a wavefront takes for eight rows
 // of 256 bfloat16 with entropy and 4 alternatives, the passes over the elements (unpack, maximum, exponential, two sums)
 // are 350.  100352 such rows: 20.4 us (2.8 TB/s); without alternatives and entropy 13 us (4.0 TB/s); 200000 x 100 float32
 // 14.4 us (5.5 TB/s).
@@ -1339,7 +1339,7 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& spa
 // Four wavefronts where there are rows or parts enough to fill the chip (several workgroups a compute unit hide each
 // other's joins), sixteen where there are few, one where there are many of moderate length.  Measured: 2048 x 65536
 // bfloat16, log-probability alone 54 us (5.0 TB/s), with entropy and 8 alternatives 66 us (4.1 TB/s; the vector units are
-// 83 % busy); float32 92 us (5.8 TB/s) and 101 us; 8192 x 4096 bfloat16 15 and 26 us; 50 x 50000 float32 with 64
+// 81 % busy); float32 92 us (5.8 TB/s) and 101 us; 8192 x 4096 bfloat16 15 and 26 us; 50 x 50000 float32 with 64
 // alternatives 15 us, bound by the latency of its phases.  Loading a round ahead gained nothing.
 template <int DT, bool ENT, bool TOP, int NT>
 __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
