@@ -673,10 +673,10 @@ __device__ __forceinline__ void small_sorted(const float* o, int V, int lane, in
   for (int j = E * L + lane; j < k; j += L) emit(j, -INFINITY, -1);
 }
 
-// Short rows, forward.  Bound by the vector units (92 % busy) and not by memory: of 743 instructions that a wavefront takes for eight rows
-// of 256 bfloat16 with entropy and 4 alternatives, the passes over the elements (unpack, maximum, exponential, two sums)
-// are 350.  100352 such rows: 20.4 us (2.8 TB/s); without alternatives and entropy 13 us (4.0 TB/s); 200000 x 100 float32
-// 14.4 us (5.5 TB/s).
+// Short rows, forward.  Bound by the vector units (92 % busy) and not by memory: of 743 instructions that a wavefront takes for
+// eight rows of 256 bfloat16 with entropy and 4 alternatives, about half are the passes over the elements (unpack,
+// maximum, exponential, two sums).  100352 such rows: 20.4 us (2.8 TB/s); without alternatives and entropy 13 us (4.0 TB/s);
+// 200000 x 100 float32 14.4 us (5.5 TB/s).
 enum { kNoTop = 0, kRanked = 1, kSorted = 2 };
 template <int DT, int VEC, int L, int SL, bool ENT, int TOP>
 __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
