@@ -464,9 +464,12 @@ __device__ __forceinline__ void small_stats(SmallRow<DT, VEC, L, SL>& x, float c
 
 // The k largest of a row held by L lanes, through emit(rank, value, index) by any lane; index -1 past the finite values.
 //
-// The k-th largest of the largest values of NB parts of every lane's elements, k <= L NB / 2, is a lower bound of the k-th
-// largest element, which little more than k elements reach.  Those go to the group's list in LDS and are ranked by
-// counting.  When the list is too short for them (many equal values): one rank at a time.
+// The k-th largest of the largest values of NB parts of every lane's elements is a lower bound of the k-th largest element.
+// With twice as many parts that hold elements as k, about 1.4 k elements reach it (the median of the parts' largest
+// values): those go to the group's list in LDS and are ranked by counting.  A row may fill a quarter of its tile only, so
+// the number of parts follows from what it fills; beyond 8 a lane the elements themselves are searched.  (10000 x 1092
+// float16, 64 alternatives: 35 us a call; 520 by two parts a lane, whose bound more elements reach than the list holds.)
+// When the list is too short all the same (many equal values): one rank at a time.
 constexpr int kSmallList = 8;            // list entries per lane
 // lanes of one wavefront that read what others of it wrote: in order without a wait
 __device__ __forceinline__ void wave_sync() {
@@ -479,18 +482,18 @@ __device__ __forceinline__ float small_bound(const float* o, int k) {
   constexpr int B = NB < E ? NB : E;          // (a tile of few elements has no more parts than those)
   float mx[B];
 #pragma unroll
-  for (int b = 0; b < B; ++b) mx[b] = max_of<E / B>(o + b * (E / B), -INFINITY);
-  if (k > kPops) {
+  for (int b = 0; b < B; ++b)
+    if constexpr (E == B) mx[b] = o[b];
+    else mx[b] = max_of<E / B>(o + b * (E / B), -INFINITY);
+  if (B > 8 || k > kPops) {
     // the bound's bits one by one, below the exponent of the largest value if k values share it, until not many more than
-    // k reach it
-    uint32_t key[B];
-    float first = mx[0];
-#pragma unroll
-    for (int b = 0; b < B; ++b) key[b] = order_key(mx[b]), first = fmaxf(first, mx[b]);
+    // k reach it (a key past that of +inf is a NaN's, which none reaches)
+    const float first = max_of<B>(mx, -INFINITY);
     auto reach = [&](uint32_t t) {
+      const float at = key_value(t);
       uint32_t c = 0;
 #pragma unroll
-      for (int b = 0; b < B; ++b) c += key[b] >= t ? 1u : 0u;
+      for (int b = 0; b < B; ++b) c += mx[b] >= at ? 1u : 0u;
       return (int)rsum_u<L>(c);
     };
     const uint32_t start = order_key(gmax<L>(first)) & 0xff800000u;
@@ -524,12 +527,18 @@ __device__ __forceinline__ float small_bound(const float* o, int k) {
   return fmaxf(bound, -3.402823466e38f);      // -inf is no alternative
 }
 template <int DT, int VEC, int L, int SL, typename Emit>
-__device__ __forceinline__ void small_top(const float* o, const char* p, int V, int lane, int k, cand_t* list, int* count, Emit emit) {
+__device__ __forceinline__ void small_top(const float* o, const char* p, int V, int n, int lane, int k, cand_t* list, int* count,
+                                          Emit emit) {
   constexpr int E = VEC * SL;
   static_assert(E <= 32, "");
   auto index = [&](int j, int e) { return slot_base<VEC>(lane + L * j, V) + e; };
   {
-    const float bound = k <= L ? small_bound<2, E, L>(o, k) : (k <= 2 * L ? small_bound<4, E, L>(o, k) : small_bound<8, E, L>(o, k));
+    // (tiles whose elements fit the list take the same number for all rows: rows of several sizes share a wavefront)
+    const int filled = E <= kSmallList ? SL * L : (n + VEC - 1) / VEC, wanted = 2 * k * SL;
+    const float bound = 2 * filled >= wanted   ? small_bound<2, E, L>(o, k)
+                        : 4 * filled >= wanted ? small_bound<4, E, L>(o, k)
+                        : 8 * filled >= wanted ? small_bound<8, E, L>(o, k)
+                                               : small_bound<32, E, L>(o, k);
     uint32_t bits = 0;
 #pragma unroll
     for (int i = E - 1; i >= 0; --i) bits = bits + bits + (o[i] >= bound ? 1u : 0u);
@@ -727,7 +736,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
       float o[E];
       x.values(o);
       if constexpr (TOP == kSorted) small_sorted<DT, VEC, L, SL>(o, V, lane, a.top, emit);
-      else small_top<DT, VEC, L, SL>(o, p, V, lane, a.top, lists[TOP == kRanked ? g : 0], &counts[g], emit);
+      else small_top<DT, VEC, L, SL>(o, p, V, n, lane, a.top, lists[TOP == kRanked ? g : 0], &counts[g], emit);
     }
   }
 }

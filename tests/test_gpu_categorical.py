@@ -927,3 +927,16 @@ def test_distillation_looks_at_weights_and_not_at_the_rows_mask(V):
     L.check(L.lib().dmv_cat_distill(C.byref(r), C.byref(tc), rows.data_ptr(), out.data_ptr(), None, None, 0, ws.data_ptr(), n,
                                     torch.cuda.current_stream().cuda_stream))
     assert torch.equal(out, loss) and torch.equal(rows, per_row)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V, top", [(132, 16), (132, 32), (264, 32), (264, 64), (300, 17), (520, 33), (520, 64), (1030, 20), (1092, 64), (1500, 64)])
+def test_alternatives_of_rows_that_fill_little_of_their_tile(V, top, dtype):
+    """a lane group's width doubles at these lengths; sizes down to none, next to full rows in the same wavefront"""
+    x = make((200, V), dtype, seed=V)
+    check_log_prob(x, top=top)
+    sizes = torch.randint(0, V + 1, (200,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(top), dtype=torch.int32)
+    sizes[:8] = torch.tensor([0, 1, top - 1, top, top + 1, 2 * top, V // 4, V], device="cuda")
+    check_log_prob(x, sizes=sizes, entropy=True, top=top, grads=True)
+    check_log_prob(-x.abs() - 1, sizes=sizes, top=top)                      # nothing but negative values
+    check_log_prob(torch.where(rand((200, V), 41) < 0.9, -math.inf, x.float()).to(dtype), sizes=sizes, top=top)
