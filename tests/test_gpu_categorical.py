@@ -940,3 +940,19 @@ def test_alternatives_of_rows_that_fill_little_of_their_tile(V, top, dtype):
     check_log_prob(x, sizes=sizes, entropy=True, top=top, grads=True)
     check_log_prob(-x.abs() - 1, sizes=sizes, top=top)                      # nothing but negative values
     check_log_prob(torch.where(rand((200, V), 41) < 0.9, -math.inf, x.float()).to(dtype), sizes=sizes, top=top)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V, rows", [(2049, 5000), (4100, 300), (66000, 8), (140001, 3), (262147, 1), (262147, 9), (600000, 3)])
+def test_alternatives_of_long_rows_with_few_elements(V, rows, dtype):
+    """sizes down to none: threads and parts of a row without elements, and a last part with a few"""
+    x = make((rows, V), dtype, seed=V)
+    sizes = (rand((rows,), rows) ** 2 * V).int() + 1
+    few = torch.tensor([V, 500, 70, 520, 1, 0, 64, 65], dtype=torch.int32, device="cuda")[:rows]
+    sizes[:len(few)] = few
+    for top in (64, 17, 3):
+        check_log_prob(x, top=top)
+        check_log_prob(x, sizes=sizes, entropy=True, top=top)
+    low = torch.where(torch.arange(V, device="cuda") < V - 40, -math.inf, x.float()).to(dtype)      # the last part's elements only
+    check_log_prob(low, top=64)
+    check_log_prob(low, sizes=sizes, top=64)
