@@ -1207,10 +1207,10 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& spa
     }
     __syncthreads();
   };
-  // f(keys that reach `lowest`, index of the slot's first element, bits of those elements) for the listed groups
-  auto each_slot = [&](uint32_t lowest, auto f) {
+  // f(keys that reach `lowest`, index of the slot's first element, bits of those elements) for the listed groups, until done()
+  auto each_slot = [&](uint32_t lowest, auto done, auto f) {
     const int total = sh.groups * gsz;
-    for (int j = tid; j < total; j += NT) {
+    for (int j = tid; j < total && !done(); j += NT) {
       const int l = j / gsz, at = sh.list[l];
       const int s = s0 + (at & (NT - 1)) + NT * (at / NT * gsz + (j - l * gsz));
       if (s >= s1) continue;
@@ -1226,9 +1226,12 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& spa
       if (bits) f(key, b, bits);
     }
   };
+  // (stops where there are more than fit: a row of equal values would add all of its slots to one counter, 300 us instead
+  // of 59 for 2048 x 65536 bfloat16)
   auto collect = [&](uint32_t lowest) {
     list_groups(lowest);
-    each_slot(lowest, [&](const uint32_t* key, int b, uint32_t bits) {
+    const volatile int* count = &sh.count;
+    each_slot(lowest, [&] { return *count > kCand; }, [&](const uint32_t* key, int b, uint32_t bits) {
       int at = atomicAdd(&sh.count, __popc(bits));
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
@@ -1342,7 +1345,7 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& spa
       cand_t last = ~0ull;
       for (done = 0; done < k; ++done) {
         cand_t best = 0;
-        each_slot(above, [&](const uint32_t* key, int b, uint32_t bits) {
+        each_slot(above, [] { return false; }, [&](const uint32_t* key, int b, uint32_t bits) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             const cand_t o = candidate(key[e], (uint32_t)(b + e));
@@ -1544,7 +1547,7 @@ static_assert(kMaxTop <= 1 << (kJoinDepths - 1), "");
 template <int DT>
 __global__ void __launch_bounds__(kJoinThreads) k_cat_fwd_join(Fwd a) {
   __shared__ cand_t cand[kMaxParts * kMaxTop + kCandPad];
-  __shared__ int count;
+  __shared__ int count, sums[2][kJoinThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const bool seen = row_seen(a.r, row);
@@ -1596,7 +1599,36 @@ __global__ void __launch_bounds__(kJoinThreads) k_cat_fwd_join(Fwd a) {
     if (o.x >= tau) cand[atomicAdd(&count, 1)] = candidate(o.x, o.y);
   }
   __syncthreads();
-  const int have = count;
+  int have = count;
+  if (have > 4 * a.top + 64) {
+    // many equal values: what reaches the k-th largest candidate or a smaller one, key and index bit by bit (8 x 262147
+    // float32 zeros, 64 alternatives: 52 us a call, 1150 with all of them ranked)
+    constexpr int MINE = kMaxParts * kMaxTop / kJoinThreads;
+    cand_t mine[MINE], least = 0;
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) mine[q] = tid + kJoinThreads * q < have ? cand[tid + kJoinThreads * q] : 0;
+    for (int bit = 63, reach = have; bit >= 0 && reach > 2 * a.top; --bit) {
+      const cand_t t = least | 1ull << bit;
+      uint32_t n = 0;
+#pragma unroll
+      for (int q = 0; q < MINE; ++q) n += mine[q] >= t ? 1u : 0u;
+      n = rsum_u<64>(n);
+      if (lane == 0) sums[bit & 1][tid >> 6] = (int)n;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < kJoinThreads / 64; ++w) all += sums[bit & 1][w];
+      if (all >= a.top) least = t, reach = all;
+    }
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < MINE; ++q)
+      if (mine[q] && mine[q] >= least) cand[atomicAdd(&count, 1)] = mine[q];
+    __syncthreads();
+    have = count;
+  }
   rank_candidates<kJoinThreads>(cand, have, a.top, [&](int rank, uint32_t key, int i) {
     a.top_idx[row * a.top + rank] = i;
     a.top_lp[row * a.top + rank] = (key_value(key) - m) - logs;

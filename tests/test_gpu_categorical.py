@@ -956,3 +956,16 @@ def test_alternatives_of_long_rows_with_few_elements(V, rows, dtype):
     low = torch.where(torch.arange(V, device="cuda") < V - 40, -math.inf, x.float()).to(dtype)      # the last part's elements only
     check_log_prob(low, top=64)
     check_log_prob(low, sizes=sizes, top=64)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V, rows", [(2049, 70), (2049, 4100), (50001, 9), (66001, 300), (262147, 8), (600000, 2)])
+def test_alternatives_of_equal_values_in_long_rows(V, rows, dtype):
+    """rows of one value (an untrained network's), of two, and of one value behind a few larger ones in every part"""
+    x = torch.zeros(rows, V, dtype=dtype, device="cuda")
+    check_log_prob(x, top=64)
+    check_log_prob(x, top=1)
+    x[:, ::3] = -1.5
+    check_log_prob(x, top=64)
+    x[:, V // 100::V // 37 + 1] = 2.0
+    check_log_prob(x, top=50, sizes=torch.full((rows,), V - 3, dtype=torch.int32, device="cuda"))
