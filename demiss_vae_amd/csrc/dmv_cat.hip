@@ -850,7 +850,9 @@ __device__ __forceinline__ void small_zeros(char* out, int V, int lane) {
 
 template <int DT, int VEC, int L, int SL, int NT>
 __global__ void __launch_bounds__(NT) k_cat_distill_small(Dist a) {
-  constexpr int E = VEC * SL, ES = sizeof(typename Elem<DT>::type), WORDS = E * L / 32, NG = NT / L;
+  // (the smallest tiles have fewer categories than a word has bits)
+  constexpr int E = VEC * SL, ES = sizeof(typename Elem<DT>::type), WORDS = (E * L + 31) / 32, NG = NT / L;
+  static_assert(WORDS >= 1 && WORDS * 32 >= E * L, "a bit for every category of the tile");
   constexpr bool LONE = NT == kLoneThreads;
   __shared__ double sums[NT / 64];
   __shared__ uint32_t given[NG][WORDS];

@@ -969,3 +969,34 @@ def test_alternatives_of_equal_values_in_long_rows(V, rows, dtype):
     check_log_prob(x, top=64)
     x[:, V // 100::V // 37 + 1] = 2.0
     check_log_prob(x, top=50, sizes=torch.full((rows,), V - 3, dtype=torch.int32, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------ more entries than categories
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [1, 2, 3, 7, 8, 10, 12, 16, 17, 31, 33])
+@pytest.mark.parametrize("k", [17, 20, 33, 64, 65, 200])
+@pytest.mark.parametrize("rows", [60, 700])
+def test_distill_more_entries_than_categories(V, k, rows, dtype):
+    """The alternatives of short rows, with nothing behind them, and entries given several times; rows of small and of
+    large |log p|, many row groups in a workgroup.  The first entry of a row is its most probable one, and in every other
+    row its least probable one, whose log p is the largest."""
+    x = make((rows, V), dtype, seed=V)
+    w = rand((rows,)) + 0.1
+    a = dmv.categorical_log_prob(make((rows, V), torch.float32, seed=k, scale=3.0), top=min(k, 64))
+    t, idx = a.top_log_prob, a.top_index
+    t, idx = torch.nn.functional.pad(t, (0, k - t.shape[1]), value=-math.inf), torch.nn.functional.pad(idx, (0, k - idx.shape[1]), value=-1)
+    have = min(V, k)
+    order = torch.arange(k, device="cuda").repeat(rows, 1)
+    order[1::2, :have] = torch.arange(have - 1, -1, -1, device="cuda")
+    t, idx = t.gather(-1, order), idx.gather(-1, order)
+    assert bool((idx[:, :have] >= 0).all()) and not bool((idx[:, have:] >= 0).any())
+    once = check_distill(x, t, idx, weight=w, T=1.5)
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(check_distill(x, t, idx, weight=w, T=1.5), once))
+    check_distill(x, t, idx, weight=w, upstream=0.5)
+    again = ints(V, (rows, k), seed=k)
+    again[rand((rows, k), 6) < 0.1] = -1
+    logits = make((rows, k), torch.float32, seed=k + 1, scale=4.0)
+    once = check_distill(x, logits, again, weight=w)
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(check_distill(x, logits, again, weight=w), once))
