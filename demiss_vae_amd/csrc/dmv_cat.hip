@@ -1250,6 +1250,7 @@ __device__ void block_top(TopShared<NT>& sh, const char* p, const Span<VEC>& spa
   auto thin_out = [&](int have) {
     constexpr int MINE = (kCand + NT - 1) / NT;
     cand_t mine[MINE];
+    __syncthreads();          // every wavefront has read the number of candidates, which is counted again
 #pragma unroll
     for (int q = 0; q < MINE; ++q) mine[q] = tid + NT * q < have ? sh.cand[tid + NT * q] : 0;
     if (tid < 64) {

@@ -1000,3 +1000,22 @@ def test_distill_more_entries_than_categories(V, k, rows, dtype):
     once = check_distill(x, logits, again, weight=w)
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(check_distill(x, logits, again, weight=w), once))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V, rows", [(3000, 700), (9000, 300), (9000, 40), (50001, 50), (262147, 5)])
+def test_alternatives_from_many_candidates(V, rows, dtype):
+    """Long rows of which 70 to 512 elements come into question, which are thinned out before they are ranked: few categories,
+    and as many among the others, by workgroups of four and of sixteen wavefronts and in parts of rows.  Every call of
+    the same rows gives the same."""
+    x = make((rows, V), dtype, seed=V)
+    few = torch.full((rows, V), -math.inf, dtype=dtype, device="cuda")
+    at = torch.argsort(rand((rows, V), 51), dim=-1)[:, :400]
+    few.scatter_(-1, at, x.gather(-1, at))
+    for z, sizes in ((x, 500), (x, 300), (few, V)):
+        sizes = torch.full((rows,), sizes, dtype=torch.int32, device="cuda")
+        for top in (64, 20, 1):
+            once = check_log_prob(z, sizes=sizes, entropy=True, top=top)
+            for _ in range(5):
+                again = dmv.categorical_log_prob(z, sizes=sizes, entropy=True, top=top)
+                assert torch.equal(again.top_index, once.top_index) and torch.equal(again.top_log_prob, once.top_log_prob)
