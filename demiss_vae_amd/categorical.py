@@ -117,7 +117,7 @@ def _set_logits(r, logits, keep):
     """The logits of a call: its rows in `r`; what they had to be copied to is kept alive with the call's other arrays."""
     flat, r.rows, _, r.ld = _rows(logits)
     r.logits = flat.data_ptr()
-    if flat is not logits:
+    if r.logits != logits.data_ptr():
         keep.append(flat)
 
 

@@ -185,3 +185,21 @@ def test_entries_refuse_rows_beyond_the_grid_of_the_widest_tile():
 def test_a_number_as_weight_is_an_argument():
     with pytest.raises(RuntimeError, match="no CPU path"):
         dmv.distill_top_logits(_logits(4, 7), torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.long), weight=0.25)
+
+
+def test_a_view_of_the_logits_is_not_held():
+    """Rows with a pitch are read where they are.  What autograd saves of them is autograd's: they may be written over
+    where its hooks have put them elsewhere, and are not kept alive; a copy that a call has made is."""
+    from types import SimpleNamespace
+    from demiss_vae_amd import categorical as cat
+    memory = torch.arange(48.0).view(4, 12)
+    for logits, copies in ((memory[:, :7], 0), (memory[:, :, None].transpose(1, 2)[:, :, 2:9], 0), (memory, 0), (memory.t(), 1),
+                           (memory.view(2, 2, 12).transpose(0, 1), 1)):
+        r, keep = cat._row_args(logits, None, None, None)
+        cat._set_logits(r, logits, keep)
+        assert len(keep) == copies
+        ctx = SimpleNamespace()
+        cat._keep(ctx, logits, r, keep)
+        saved = logits.clone()
+        memory.add_(1.0)
+        assert cat._kept(ctx, saved)[0].V == logits.shape[-1]
