@@ -124,7 +124,7 @@ def _set_logits(r, logits, keep):
 def _keep(ctx, logits, r, keep):
     """What a backward pass needs of a call's arguments.  Its arrays are held here, and their versions, because pointers to
     them are: saved tensors may come back from elsewhere, and may not have been made for saving (a teacher's, say)."""
-    ctx.kept = r, keep, _versions(keep), r.logits == logits.data_ptr()
+    ctx.kept = r, keep, _versions(keep), logits.stride() if r.logits == logits.data_ptr() else None
 
 
 def _versions(keep):
@@ -136,11 +136,11 @@ def _versions(keep):
 
 def _kept(ctx, logits):
     """The call's rows for its backward pass, with the saved logits where they are now; and what has to stay alive."""
-    r, keep, versions, in_place = ctx.kept
+    r, keep, versions, strides = ctx.kept
     if _versions(keep) != versions:
         raise RuntimeError("a tensor that the gradient of a categorical operator needs (X, M, sizes, weight or the teacher's) "
                            "was modified in place after the forward call")
-    if not in_place or r.logits == logits.data_ptr():
+    if strides is None or (r.logits == logits.data_ptr() and strides == logits.stride()):
         return r, None
     r, moved = L.DmvCatRows.from_buffer_copy(r), []
     _set_logits(r, logits, moved)

@@ -203,3 +203,31 @@ def test_a_view_of_the_logits_is_not_held():
         saved = logits.clone()
         memory.add_(1.0)
         assert cat._kept(ctx, saved)[0].V == logits.shape[-1]
+
+
+# ------------------------------------------------------------------------------------------ what a backward pass holds
+def _held(logits):
+    from types import SimpleNamespace
+    from demiss_vae_amd import categorical as cat
+    r, keep = cat._row_args(logits, None, None, None)
+    cat._set_logits(r, logits, keep)
+    ctx = SimpleNamespace()
+    cat._keep(ctx, logits, r, keep)
+    return lambda saved: cat._kept(ctx, saved)[0]
+
+
+@pytest.mark.parametrize("ours, back", [((12, 1), (7, 1)), ((7, 1), (12, 1)), ((12, 1), (1, 4)), ((0, 1), (7, 1))])
+def test_saved_logits_of_another_pitch_at_the_same_address(ours, back):
+    """Logits that autograd's hooks hand back may lie where the first ones lay (that memory is free again) in rows of
+    another pitch."""
+    memory = torch.arange(48.0)
+    first, again = memory.as_strided((4, 7), ours), memory.as_strided((4, 7), back)
+    kept = _held(first)
+    same = kept(first)
+    assert (same.logits, same.ld, same.rows, same.V) == (first.data_ptr(), ours[0], 4, 7)
+    r = kept(again)
+    assert (r.rows, r.V) == (4, 7)
+    if back[1] == 1:
+        assert (r.logits, r.ld) == (again.data_ptr(), back[0])
+    else:
+        assert r.logits != again.data_ptr() and r.ld == 7       # copied to rows

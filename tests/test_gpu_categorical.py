@@ -1019,3 +1019,32 @@ def test_alternatives_from_many_candidates(V, rows, dtype):
             for _ in range(5):
                 again = dmv.categorical_log_prob(z, sizes=sizes, entropy=True, top=top)
                 assert torch.equal(again.top_index, once.top_index) and torch.equal(again.top_log_prob, once.top_log_prob)
+
+
+@pytest.mark.parametrize("V", [40, 5000, 90000])
+def test_saved_logits_come_back_to_the_same_address(V):
+    """... in rows of another pitch: what a hook kept elsewhere may get the memory of the first logits again"""
+    x, losses = _losses(V)
+    for f in losses:
+        z = x.clone().requires_grad_()
+        (want,) = torch.autograd.grad(f(1.0 * z), z)
+        memory = torch.empty(4 * (V + 9), device="cuda")
+        for ours, back in ((V + 9, V), (V, V + 9)):
+            def pack(t):
+                return t.clone()
+
+            def unpack(t):
+                if t.shape != (4, V):
+                    return t
+                again = memory.as_strided((4, V), (back, 1))
+                return again.copy_(t)
+
+            y = memory.as_strided((4, V), (ours, 1))
+            y.copy_(x)
+            y.requires_grad_()
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                loss = f(y)
+            memory.fill_(7.0)
+            (got,) = torch.autograd.grad(loss, y)
+            assert torch.equal(got, want)
+            memory = torch.empty(4 * (V + 9), device="cuda")
