@@ -11,12 +11,13 @@ another model gave:
     loss, kl = distill_top_logits(logits, teacher.top_log_prob, teacher.top_index, sizes=sizes, weight=(~M).float())
     log_px = (categorical_log_prob(logits, X, M, sizes=sizes).log_prob).sum(-1)
 
-Both are differentiable with respect to the logits (float32, bfloat16 or float16), run on the current stream, allocate
-through torch only and record into HIP graphs.  There is no CPU path."""
+Both are differentiable with respect to the logits (float32, bfloat16 or float16), in reverse mode and once, run on the
+current stream, allocate through torch only and record into HIP graphs.  There is no CPU path."""
 import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -79,6 +80,15 @@ def _check_logits(logits):
 def _need_gpu(logits):
     if not logits.is_cuda:
         raise RuntimeError(f"the categorical operators have no CPU path: the logits are on {logits.device}")
+
+
+def _no_tangent(*tensors):
+    """Forward-mode gradients are not formed; inside a forward-mode level a tensor that carries one is refused."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the categorical operators have no forward-mode gradient")
 
 
 def _integers(t, what):
@@ -241,6 +251,7 @@ def categorical_log_prob(logits, X=None, M=None, *, sizes=None, entropy=False, t
     are not looked at.  top: 0 .. 64; equal logits rank by their index, and places past the categories of non-zero
     probability hold -1 and -inf.  Results are float32.  log_prob, entropy and top_log_prob are differentiable."""
     _check_logits(logits)
+    _no_tangent(logits)
     top = int(top)
     if not 0 <= top <= L.CAT_MAX_TOP:
         raise ValueError(f"top = {top}: 0 .. {L.CAT_MAX_TOP}")
@@ -331,6 +342,7 @@ def distill_top_logits(logits, top_logits, top_index, *, sizes=None, weight=None
         weight = torch.full((), float(weight), device=logits.device)
     if torch.is_grad_enabled() and (top_logits.requires_grad or (weight is not None and weight.requires_grad)):
         raise ValueError("the teacher's logits and the weights have no gradient: detach them")
+    _no_tangent(logits, top_logits, weight)
     k = top_logits.shape[-1]
     if not 1 <= k <= L.CAT_MAX_TEACHER:
         raise ValueError(f"{k} entries per row: 1 .. {L.CAT_MAX_TEACHER}")

@@ -231,3 +231,31 @@ def test_saved_logits_of_another_pitch_at_the_same_address(ours, back):
         assert (r.logits, r.ld) == (again.data_ptr(), back[0])
     else:
         assert r.logits != again.data_ptr() and r.ld == 7       # copied to rows
+
+
+# ------------------------------------------------------------------------------------------ forward-mode gradients
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_gradients_are_refused(grad):
+    """A tangent of the logits, of the teacher's or of the weights would be dropped."""
+    import torch.autograd.forward_ad as fw
+    idx = torch.zeros(4, 2, dtype=torch.long)
+    with fw.dual_level():
+        x = fw.make_dual(_logits(4, 7).requires_grad_(grad), torch.ones(4, 7))
+        t, w = fw.make_dual(torch.zeros(4, 2), torch.ones(4, 2)), fw.make_dual(torch.ones(4), torch.ones(4))
+        for no_grad in (False, True):
+            with torch.set_grad_enabled(not no_grad):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    dmv.categorical_log_prob(x, entropy=True)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    dmv.distill_top_logits(x, torch.zeros(4, 2), idx)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    dmv.distill_top_logits(_logits(4, 7), t, idx)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    dmv.distill_top_logits(_logits(4, 7), torch.zeros(4, 2), idx, weight=w)
+        # without a tangent they are ordinary arguments
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            dmv.categorical_log_prob(_logits(4, 7), entropy=True)
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            dmv.distill_top_logits(_logits(4, 7), torch.zeros(4, 2), idx, weight=0.5)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda z: dmv.categorical_log_prob(z, entropy=True).entropy, (_logits(4, 7),), (torch.ones(4, 7),))
