@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_fwd_small(Fwd a) {
   const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
   const float H = empty ? 0.f : fmaf(kLn2 * u, inv_s, logs);
   if (lane == 0) {
-    if (a.log_prob) a.log_prob[(uint32_t)row] = !seen ? 0.f : (!given ? NAN : (empty ? -INFINITY : (xX - m) - logs));
+    if (a.log_prob) a.log_prob[(uint32_t)row] = !seen ? 0.f : (empty ? -INFINITY : (!given ? NAN : (xX - m) - logs));
     if (ENT) a.entropy[(uint32_t)row] = H;
     if (a.stats) a.stats[(uint32_t)row] = f32x4{m, inv_s, logs, H};
   }
@@ -1510,7 +1510,7 @@ __global__ void __launch_bounds__(NT) k_cat_fwd_row(Fwd a) {
       float lp = 0.f;
       if (seen) {
         const int64_t X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
-        lp = (X < 0 || X >= n) ? NAN : (empty ? -INFINITY : (Elem<DT>::load(p, X) - m) - logs);
+        lp = empty ? -INFINITY : ((X < 0 || X >= n) ? NAN : (Elem<DT>::load(p, X) - m) - logs);
       }
       a.log_prob[row] = lp;
     }
@@ -1568,7 +1568,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_cat_fwd_join(Fwd a) {
       float lp = 0.f;
       if (seen) {
         const int64_t X = a.r.X[wrap(row, a.r.x_period, a.r.rows)];
-        lp = (X < 0 || X >= n) ? NAN : (empty ? -INFINITY : (Elem<DT>::load(p, X) - m) - logs);
+        lp = empty ? -INFINITY : ((X < 0 || X >= n) ? NAN : (Elem<DT>::load(p, X) - m) - logs);
       }
       a.log_prob[row] = lp;
     }

@@ -518,9 +518,10 @@ int dmv_grid_divergences(int32_t gen_dist, int32_t D, int32_t Zd, int64_t Nz, co
  *   reads X[r % x_period] (the given category), M[r % m_period] (NULL: all seen; a row that is not seen has
  *   log-probability 0 whatever X holds), sizes[r % size_period] (NULL: V; categories >= size do not exist, whatever
  *   their logits hold; clamped to 0..V).
- * A row without any category of non-zero probability (size 0, or all logits -inf) has entropy 0, log-probability -inf,
- * no alternatives and a zero gradient.  NaN or +inf among a row's logits makes its outputs NaN (alternatives -1); a given
- * category outside the row's, where it is seen, makes that row's log-probability and gradient NaN.
+ * A row without any category of non-zero probability (size 0, or all logits -inf) has entropy 0, log-probability -inf
+ * (whatever category is given), no alternatives and a zero gradient.  NaN or +inf among a row's logits makes its outputs NaN
+ * (alternatives -1); a given category outside another row's, where it is seen, makes that row's log-probability and gradient
+ * NaN.
  * Limits (DMV_E_UNSUPPORTED): fewer than 2^26 - 4 rows (2^24 where V > DMV_CAT_SHORT_ROW), V below 2^31 - 2^20. */
 enum { DMV_F32 = 0, DMV_BF16 = 1, DMV_F16 = 2 };
 #define DMV_CAT_MAX_TOP 64

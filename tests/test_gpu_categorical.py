@@ -1048,3 +1048,35 @@ def test_saved_logits_come_back_to_the_same_address(V):
             (got,) = torch.autograd.grad(loss, y)
             assert torch.equal(got, want)
             memory = torch.empty(4 * (V + 9), device="cuda")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [3, 40, 1000, 2000, 5000, 70000, 262147])
+@pytest.mark.parametrize("rows", [8, 300])
+def test_observed_entries_without_categories(V, rows, dtype):
+    """Rows of size 0 and rows of nothing but -inf that are observed: -inf and a zero gradient, whatever category is given; a
+    category that is none of the row's shows in every other row."""
+    rows = min(rows, 20_000_000 // V)
+    x = make((rows, V), dtype, seed=V)
+    sizes = torch.full((rows,), V, dtype=torch.int32, device="cuda")
+    X = ints(V, (rows,))
+    sizes[:3] = torch.tensor([0, 0, -5], device="cuda")
+    X[:3] = torch.tensor([0, V, -1], device="cuda")
+    x[3:6] = -math.inf
+    sizes[4] = V - 1
+    X[3:6] = torch.tensor([0, V - 1, -1], device="cuda")
+    sizes[6] = V - 1
+    X[6] = V - 1
+    for top in (0, min(V, 5)):
+        for entropy in (False, True):
+            z = x.clone().requires_grad_()
+            got = dmv.categorical_log_prob(z, X, sizes=sizes, entropy=entropy, top=top)
+            assert bool((got.log_prob[:6] == -math.inf).all()) and bool(got.log_prob[6].isnan())
+            assert bool(torch.isfinite(got.log_prob[7:]).all())
+            (dx,) = torch.autograd.grad(got.log_prob.sum(), z)
+            assert not bool(dx[:6].any()) and bool(dx[6, :V - 1].isnan().all()) and float(dx[6, V - 1]) == 0.0
+            assert bool(torch.isfinite(dx[7:]).all())
+            if entropy:
+                assert not bool(got.entropy[:6].any())
+            if top:
+                assert bool((got.top_index[:6] == -1).all()) and bool((got.top_log_prob[:6] == -math.inf).all())
