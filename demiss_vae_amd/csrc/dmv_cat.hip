@@ -822,7 +822,8 @@ __global__ void __launch_bounds__(kSmallThreads) k_cat_bwd_small(Bwd a) {
 
 // ------------------------------------------------------------------------------------------ distillation, shared parts
 // Teacher entry j counts if its index is not negative and its logit not -inf; the counted ones are normalised among
-// themselves.  An index past the row's categories, or a logit that is NaN or +inf, makes the row's loss and gradient NaN.
+// themselves.  An index past the row's categories, or a logit that is NaN or +inf, makes the row's loss NaN, and its gradient
+// at all of the row's categories; past those a gradient is 0 whatever the row holds.
 __device__ __forceinline__ bool entry_counts(float t, int64_t i) { return i >= 0 && t != -INFINITY; }
 
 __device__ __forceinline__ float exp_hw(float x) { return exp2_hw(x * kLog2e); }
@@ -889,7 +890,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_small(Dist a) {
       small_stats<false, true>(x, a.t.c, m, r, u, kept);      // (twice the registers of the packed row, but no second exp2)
       const bool empty = m == -INFINITY && !(r != r);
       const float logs = empty ? 0.f : log1p_row(r), inv_s = empty ? 0.f : __builtin_amdgcn_rcpf(1.f + r);
-      const bool live = any && !empty;
+      const bool live = any && (!empty || bad);
       if (live && !bad) {
         float s = 0.f, held = 0.f;
         for (int j = lane; j < K; j += L)
@@ -920,7 +921,12 @@ __global__ void __launch_bounds__(NT) k_cat_distill_small(Dist a) {
           if (fst >= V || !live) continue;
           float v[VEC];
   #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[e] = f * kept[j * VEC + e];     // (what does not count: 0)
+          for (int e = 0; e < VEC; ++e) v[e] = f * kept[j * VEC + e];     // (what does not count: 0, or NaN)
+          if (!(fabsf(f) < INFINITY)) {
+            const int b = slot_base<VEC>(lane + L * j, V);
+  #pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = b + e < n ? v[e] : 0.f;
+          }
           if (fst + VEC <= V) slot_store<DT, VEC>(out, fst, v);
           else {
   #pragma unroll
@@ -1873,7 +1879,7 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
     a.loss_part[row] = (double)w * (double)kl;
   }
   if (!a.d) return;
-  if (!te.any || empty) {
+  if (!te.any || (empty && !te.bad)) {
     zeros();
     return;
   }
@@ -1887,6 +1893,10 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = exp2_hw((v[e] - m) * a.t.c) * f;
     const int b = span.base(s);
+    if (!(fabsf(f) < INFINITY)) {        // past the row's size 0 all the same
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = b + e < n ? v[e] : 0.f;
+    }
     if (span.whole(s)) slot_store<DT, VEC>(out, b, v);
     else {
 #pragma unroll
@@ -1966,7 +1976,7 @@ __global__ void __launch_bounds__(kRowThreads) k_cat_distill_chunk(Dist a) {
         sp.p[tid] = te.p;
         sp.i[tid] = te.i;
       }
-      live = te.any && st[1] != 0.f;
+      live = te.any && (st[1] != 0.f || te.bad);
     }
     const float scale = te.bad ? NAN : gs * w * a.t.inv_T, f = scale * st[1];
 #pragma unroll

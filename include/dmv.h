@@ -558,10 +558,12 @@ int dmv_cat_log_prob_backward(const DmvCatRows* r, const float* stats, const flo
  * r % period (an entry with a negative index or a logit of -inf is empty; a category given twice counts twice) and q =
  * softmax(row / T) over all of the row's categories,
  *   per_row[r] = KL(p || q) = sum_j p_j (log p_j - log q_index[j]),   loss = sum_r weight[r % w_period] per_row[r]
- * (weight NULL: 1; X and M of the rows are not looked at).  Rows of weight 0 are not read and have per_row 0; rows without entries have 0.  d_logits (nullable)
- * receives the gradient of loss: weight / T (q - p).  An index at or past the row's size, or a logit of NaN or +inf,
- * makes the row's loss and gradient NaN; categories of probability 0 under q with p > 0 make the loss inf.  The sum of
- * the loss has a fixed order and is held in 64 bits.
+ * (weight NULL: 1; X and M of the rows are not looked at).  Rows of weight 0 are not read and have per_row 0; rows without
+ * entries have 0.  d_logits (nullable) receives the gradient of loss: weight / T (q - p), 0 past a row's size whatever the row.
+ * An index at or past the row's size, or a teacher's logit of NaN or +inf, makes the row's loss NaN and its gradient NaN at
+ * all of the row's categories; a NaN or +inf among the row's own logits makes both NaN too.  Categories of probability 0
+ * under q with p > 0 make the loss inf; in a row without any category of non-zero probability it is inf with a zero gradient.
+ * The sum of the loss has a fixed order and is held in 64 bits.
  * stats: needed by the backward call for V > DMV_CAT_SHORT_ROW ([rows][4], 16-byte aligned), nullable.
  * ws: dmv_cat_distill_ws_bytes bytes, 16-byte aligned (may be 0). */
 typedef struct DmvCatTeacher {

@@ -1080,3 +1080,44 @@ def test_observed_entries_without_categories(V, rows, dtype):
                 assert not bool(got.entropy[:6].any())
             if top:
                 assert bool((got.top_index[:6] == -1).all()) and bool((got.top_log_prob[:6] == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("V", [2, 3, 9, 40, 300, 1000, 2000, 2600, 9001, 70000, 200001])
+@pytest.mark.parametrize("rows", [12, 300])
+def test_distill_invalid_rows_with_sizes(V, rows, dtype):
+    """What makes a row NaN makes its gradient NaN at each of its categories, and leaves 0 past its size, by every kernel and
+    for every upstream gradient; a row without categories has a loss to tell and nothing to write."""
+    rows = min(rows, 20_000_000 // V)
+    x = make((rows, V), dtype, seed=V)
+    k = 2 if V < 40 else 20
+    sizes = torch.full((rows,), V - 1, dtype=torch.int32, device="cuda")
+    t, idx = teacher_of(x[:, :V - 1], min(k, V - 1), dtype=torch.float32)
+    t, idx = torch.nn.functional.pad(t, (0, k - t.shape[1]), value=-math.inf), torch.nn.functional.pad(idx, (0, k - idx.shape[1]), value=-1)
+    w = rand((rows,)) + 0.1
+    x[:, V - 1] = math.inf                              # past the size: not looked at
+    idx[0, 0] = V - 1                                   # an index past the row's size
+    t[1, 0] = math.nan
+    t[2, 0] = math.inf
+    x[3, 0] = math.nan
+    x[4, V - 2] = math.inf
+    x[5, :V - 1] = -math.inf                            # no probability anywhere ...
+    x[6, :V - 1] = -math.inf
+    idx[6, 0] = V - 1                                   # ... and an index past the row's size
+    sizes[7] = 0                                        # no categories, and so every index past the row's size
+    sizes[8] = 0
+    idx[8] = -1                                         # ... and no entries either
+    w[9] = math.nan
+    for up in (None, 0.5, math.inf):
+        z = x.clone().requires_grad_()
+        loss, per_row = dmv.distill_top_logits(z, t, idx, sizes=sizes, weight=w)
+        (dx,) = torch.autograd.grad(loss if up is None else loss * up, z)
+        assert per_row[[0, 1, 2, 3, 4, 6, 7]].isnan().all() and float(per_row[5]) == math.inf and float(per_row[8]) == 0.0
+        assert bool(torch.isfinite(per_row[9:]).all()) and bool(loss.isnan())
+        past = torch.arange(V, device="cuda") >= sizes[:, None]
+        assert not bool(dx[past].any())
+        nan = dx[:, :V - 1].isnan()
+        assert nan[[0, 1, 2, 3, 4, 6, 9]].all(), nan.float().mean(-1)[:10]
+        assert not bool(dx[[7, 8]].any())
+        if up != math.inf:
+            assert not bool(dx[5].any()) and bool(torch.isfinite(dx[10:]).all())
