@@ -922,17 +922,16 @@ __global__ void __launch_bounds__(NT) k_cat_distill_small(Dist a) {
           float v[VEC];
   #pragma unroll
           for (int e = 0; e < VEC; ++e) v[e] = f * kept[j * VEC + e];     // (what does not count: 0, or NaN)
-          if (!(fabsf(f) < INFINITY)) {
-            const int b = slot_base<VEC>(lane + L * j, V);
-  #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = b + e < n ? v[e] : 0.f;
-          }
           if (fst + VEC <= V) slot_store<DT, VEC>(out, fst, v);
           else {
   #pragma unroll
             for (int e = 0; e < VEC; ++e)
               if (V - VEC + e >= fst) Elem<DT>::store(out, V - VEC + e, v[e]);
           }
+        }
+        if (live && !(fabsf(f) < INFINITY)) {       // past the row's size 0 all the same
+          wave_sync();
+          for (int i = n + lane; i < V; i += L) Elem<DT>::store(out, i, 0.f);
         }
         if (live && !bad) {
           // A category given more than once has all its entries' probability in each of them.  Whether there is one is told
@@ -1893,10 +1892,6 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = exp2_hw((v[e] - m) * a.t.c) * f;
     const int b = span.base(s);
-    if (!(fabsf(f) < INFINITY)) {        // past the row's size 0 all the same
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = b + e < n ? v[e] : 0.f;
-    }
     if (span.whole(s)) slot_store<DT, VEC>(out, b, v);
     else {
 #pragma unroll
@@ -1904,7 +1899,9 @@ __global__ void __launch_bounds__(NT) k_cat_distill_row(Dist a) {
         if (span.holds(s, b + e)) Elem<DT>::store(out, b + e, v[e]);
     }
   }
-  __syncthreads();          // the dense part before the teacher's categories are written again
+  __syncthreads();          // the dense part before what is written again
+  if (!(fabsf(f) < INFINITY))        // past the row's size 0 all the same
+    for (int i = n + tid; i < V; i += NT) Elem<DT>::store(out, i, 0.f);
   if (te.i >= 0 && !te.bad) Elem<DT>::store(out, te.i, scale * q_minus_p(lq, share_of(sp, a.t.k, te)));
 }
 
