@@ -250,7 +250,8 @@ def categorical_log_prob(logits, X=None, M=None, *, sizes=None, entropy=False, t
     has log-probability 0 whatever its X holds; sizes (integers): the number of categories of a row, the logits past it
     are not looked at.  top: 0 .. 64; equal logits rank by their index, and places past the categories of non-zero
     probability hold -1 and -inf.  An observed entry whose X is none of its categories is NaN; one that has no category of
-    non-zero probability at all is -inf, with entropy 0 and a zero gradient.  Results are float32.  log_prob, entropy and top_log_prob are differentiable."""
+    non-zero probability at all is -inf, with entropy 0 and a zero gradient.  Results are float32.  log_prob, entropy and
+    top_log_prob are differentiable."""
     _check_logits(logits)
     _no_tangent(logits)
     top = int(top)
